@@ -339,6 +339,57 @@ int kvcu_mla_decode_noalloc(kvcu_pool* pool, uint32_t layer, uint32_t n, const u
                             const uint32_t* lens, const float* q, uint32_t n_heads, float scale,
                             float* out, void* stream);
 
+/* ------------------------------------------------------------ rotary positions
+ * y = m R(pos) x over the pairs of a head's rotary part: pair i is turned by
+ * pos * f_i (src/math.zig:197-240 is the plain interleaved form).  A kvcu_rope
+ * holds the frequencies of one model; it is immutable, host-only, and may be
+ * used from several threads, streams and devices.
+ *   rot_dim   rotated elements of a head, even, 2 .. 256; heads with an
+ *             unrotated part pass the address of the rotated one
+ *   layout    KVCU_ROPE_INTERLEAVED: pairs (2i, 2i+1); KVCU_ROPE_HALF: (i, i + rot_dim/2)
+ *   scaling   KVCU_ROPE_NONE    f_i = base^(-2i/rot_dim)
+ *             KVCU_ROPE_LINEAR  f_i / factor (position interpolation)
+ *             KVCU_ROPE_NTK     base * factor^(rot_dim/(rot_dim-2)) in place of base
+ *             KVCU_ROPE_YARN    f_i / factor for pairs that turn less than beta_slow
+ *                               times over orig_ctx positions, f_i for those that turn
+ *                               more than beta_fast times, a linear ramp over the pairs
+ *                               between (YaRN, Peng et al. 2023)
+ *   base > 1, factor >= 1; beta_fast / beta_slow: 0 = 32 / 1
+ *   mscale    magnitude m; 0 = 0.1 ln(factor) + 1 with YARN, else 1
+ * kvcu_rope_create returns NULL (and sets the last error) on anything else. */
+#define KVCU_ROPE_INTERLEAVED 0u
+#define KVCU_ROPE_HALF 1u
+#define KVCU_ROPE_NONE 0u
+#define KVCU_ROPE_LINEAR 1u
+#define KVCU_ROPE_NTK 2u
+#define KVCU_ROPE_YARN 3u
+#define KVCU_ROPE_MAX_PAIRS 128u
+#define KVCU_DTYPE_F32 0
+#define KVCU_DTYPE_BF16 1
+#define KVCU_DTYPE_F16 2
+typedef struct {
+  uint32_t rot_dim, layout, scaling, orig_ctx;
+  double base, factor, beta_fast, beta_slow, mscale;
+} kvcu_rope_desc;
+typedef struct kvcu_rope kvcu_rope;
+kvcu_rope* kvcu_rope_create(const kvcu_rope_desc* desc);
+int kvcu_rope_destroy(kvcu_rope* rope);
+/* The rot_dim/2 frequencies (radians per position) and the magnitude; either may be NULL. */
+int kvcu_rope_frequencies(const kvcu_rope* rope, double* inv_freq, double* mscale);
+/* Rotate the heads of n tokens at positions[n] (device), q and k in one launch:
+ * element e of head h of token t is at x[t*row_stride + h*head_stride + e], x
+ * the start of the rotated part, strides in elements (any order; inputs may
+ * repeat a head with stride 0).  q_heads or k_heads may be 0.  Angles are
+ * formed in 64 bits, the rotation in 32, rounded once to dtype.  transpose != 0
+ * applies m R(pos)^T, the gradient.  An output may be its own input with the
+ * same strides (in place); other overlaps of outputs with inputs are not
+ * supported, and outputs whose strides overlap are refused.  Stream-ordered. */
+int kvcu_rope_apply(const kvcu_rope* rope, int device, int dtype, int transpose, uint32_t n,
+                    const uint32_t* positions, const void* q, uint32_t q_heads, uint64_t q_row_stride,
+                    uint64_t q_head_stride, void* q_out, uint64_t q_out_row_stride, uint64_t q_out_head_stride,
+                    const void* k, uint32_t k_heads, uint64_t k_row_stride, uint64_t k_head_stride, void* k_out,
+                    uint64_t k_out_row_stride, uint64_t k_out_head_stride, void* stream);
+
 /* ------------------------------------------------------------ checkpoint I/O
  * Bytes of the pool section of a v1 checkpoint in the reference's order
  * (src/kv_cache.zig:484-492): Q8_0 -> all [rows][ceil(kv_rank/32)] 34-byte

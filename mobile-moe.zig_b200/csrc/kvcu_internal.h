@@ -60,6 +60,14 @@ struct kvcu_decode_ws {
   int last_impl;             // the kernel the last decode used
 };
 
+// Rotary frequencies (kvcu_rope.cu); immutable once created.
+struct kvcu_rope {
+  uint32_t rot, layout;
+  double mscale;
+  double inv_freq[KVCU_ROPE_MAX_PAIRS];  // radians per position of pair i
+  double turns[KVCU_ROPE_MAX_PAIRS];     // inv_freq / (2 pi)
+};
+
 // ---- programmatic dependent launch ----
 // A kernel launched with kvcu_launch_pdl may start while its predecessor in the
 // stream is still finishing (once every predecessor CTA has triggered or

@@ -38,6 +38,18 @@ class KVCudaError(RuntimeError):
         super().__init__(f"{what}: {self.name} ({code}): {detail}")
 
 
+ROPE_LAYOUTS = {"interleaved": 0, "half": 1}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+
+
+class RopeDesc(C.Structure):
+    _fields_ = [
+        ("rot_dim", C.c_uint32), ("layout", C.c_uint32), ("scaling", C.c_uint32), ("orig_ctx", C.c_uint32),
+        ("base", C.c_double), ("factor", C.c_double), ("beta_fast", C.c_double), ("beta_slow", C.c_double),
+        ("mscale", C.c_double),
+    ]
+
+
 class PoolDesc(C.Structure):
     _fields_ = [
         ("n_layers", C.c_uint32), ("num_blocks", C.c_uint32), ("block_size", C.c_uint32),
@@ -90,6 +102,11 @@ _SIGS = {
     "kvcu_decode_ws_test_withhold": (_i32, [_vp, _u32]),
     "kvcu_decode_last_impl": (_i32, [_vp]),
     "kvcu_mla_decode_noalloc": (_i32, [_vp, _u32, _u32, _vp, _u32, _vp, _vp, _vp, _vp, _u32, _f32, _vp, _vp]),
+    "kvcu_rope_create": (_vp, [C.POINTER(RopeDesc)]),
+    "kvcu_rope_destroy": (_i32, [_vp]),
+    "kvcu_rope_frequencies": (_i32, [_vp, _vp, _vp]),
+    "kvcu_rope_apply": (_i32, [_vp, _i32, _i32, _i32, _u32, _vp, _vp, _u32, _u64, _u64, _vp, _u64, _u64, _vp, _u32,
+                               _u64, _u64, _vp, _u64, _u64, _vp]),
     "kvcu_pool_read_checkpoint": (_i32, [_vp, _u64, _u64, _vp, _vp]),
     "kvcu_pool_write_checkpoint": (_i32, [_vp, _u64, _u64, _vp, _vp]),
     "kvcu_synth_rows": (_i32, [_u64, _u64, _u32, _vp, _vp, _u32, _f32, _vp, _vp]),
@@ -426,6 +443,82 @@ def prefill_synthetic(pool: DevicePool, layer, lens, table_offsets, tables, seed
         synth_rows(seed, g, t_d, p_d, W, rows[:n], outlier_p, stream)
         pool.append(layer, rows[:n], s_d, p_d, table_offsets, tables, lens=lens_dev, stream=stream)
     return total
+
+
+# ------------------------------------------------------------------ rotary positions
+class Rope:
+    """kvcu_rope: the rotary frequencies of one model (plain, linear, NTK or YaRN scaled)."""
+
+    def __init__(self, rot_dim, layout="interleaved", base=10000.0, scaling="none", factor=1.0, orig_ctx=0,
+                 beta_fast=0.0, beta_slow=0.0, mscale=0.0):
+        if layout not in ROPE_LAYOUTS or scaling not in ROPE_SCALINGS:
+            raise ValueError(f"Rope: layout {layout!r} / scaling {scaling!r}")
+        desc = RopeDesc(rot_dim, ROPE_LAYOUTS[layout], ROPE_SCALINGS[scaling], orig_ctx, base, factor, beta_fast,
+                        beta_slow, mscale)
+        self._h = lib().kvcu_rope_create(C.byref(desc))
+        if not self._h:
+            raise KVCudaError(-11, "kvcu_rope_create", last_error())
+        self.rot_dim = rot_dim
+
+    @property
+    def handle(self):
+        return self._h
+
+    def close(self):
+        if getattr(self, "_h", None):
+            lib().kvcu_rope_destroy(self._h)
+        self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def frequencies(self):
+        """(radians per position of each pair, magnitude)."""
+        f, m = np.zeros(self.rot_dim // 2, np.float64), np.zeros(1, np.float64)
+        check(lib().kvcu_rope_frequencies(self._h, _np_ptr(f), _np_ptr(m)), "kvcu_rope_frequencies")
+        return f, float(m[0])
+
+    def apply(self, positions, q=None, k=None, q_out=None, k_out=None, transpose=False, stream=None):
+        """Rotate q and / or k, [n][heads][rot_dim] CUDA tensors (any row and head strides; f32, bf16
+        or f16), by `positions` (int32 / uint32 [n]), into q_out / k_out (default: in place).
+        transpose: the gradient of the rotation."""
+        n, args, first = positions.shape[0], [], None
+        for x, y in ((q, q_out), (k, k_out)):
+            if x is None:
+                args += (None, 0, 0, 0, None, 0, 0)
+                continue
+            y = x if y is None else y
+            first = x if first is None else first
+            if x.dim() != 3 or x.shape != y.shape or x.shape[0] != n or x.shape[2] != self.rot_dim:
+                raise ValueError(f"Rope.apply: [{n}][heads][{self.rot_dim}] expected, got {tuple(x.shape)} -> "
+                                 f"{tuple(y.shape)}")
+            xs, ys = x.stride(), y.stride()
+            if xs[2] != 1 or ys[2] != 1 or not x.dtype == y.dtype == first.dtype or not x.is_cuda:
+                raise ValueError("Rope.apply: CUDA tensors of one dtype, contiguous in the last dimension")
+            if not x.device == y.device == positions.device:
+                raise ValueError("Rope.apply: tensors of different devices")
+            args += (x.data_ptr(), x.shape[1], xs[0], xs[1], y.data_ptr(), ys[0], ys[1])
+        if first is None:
+            return
+        if positions.element_size() != 4 or not positions.is_contiguous():
+            raise ValueError("Rope.apply: positions must be contiguous 32-bit integers")
+        dtype = _dtype_code(first)
+        rc = lib().kvcu_rope_apply(self._h, first.device.index, dtype, 1 if transpose else 0, n, positions.data_ptr(),
+                                   *args, _stream(stream))
+        if rc:
+            check(rc, "kvcu_rope_apply")
+
+
+def _dtype_code(t) -> int:
+    import torch
+
+    codes = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    if t.dtype not in codes:
+        raise ValueError(f"dtype {t.dtype}: float32, bfloat16 or float16 expected")
+    return codes[t.dtype]
 
 
 # ------------------------------------------------------------------ host mirror
