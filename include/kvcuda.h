@@ -339,6 +339,64 @@ int kvcu_mla_decode_noalloc(kvcu_pool* pool, uint32_t layer, uint32_t n, const u
                             const uint32_t* lens, const float* q, uint32_t n_heads, float scale,
                             float* out, void* stream);
 
+/* ------------------------------------------------------------ a bounded cache
+ * Keeping a long context under a budget of rows: kvcu_attn_mass adds up, per
+ * cached position, the attention weight it received; kvcu_evict_select picks
+ * the positions that stay; kvcu_evict_compact moves their rows to the front of
+ * their sequences.  No counterpart in the reference, whose cache only grows.
+ * All pointers are device pointers, all calls stream-ordered. */
+
+/* The attention weight of every cached position of layer `layer`, added to the
+ * running sums mass[b * mass_stride + p] (f32):
+ *   mass[b][p] = (p < old_lens[b] ? decay * mass[b][p] : 0)
+ *     + sum over i < n_q, h < n_heads of exp(scale * q[b][i][h] . row_p - lse[b][i][h])
+ * for p < len (the sequence's lens[s], or the causal plan's entry length).  The
+ * n_q queries of an entry are those of its newest positions: query i sees
+ * p < len - (n_q - 1 - i), and lse is the log-sum-exp of its scaled scores
+ * (kvcu_mla_decode_lse; -inf: a query that saw nothing adds nothing).  n_q = 1
+ * is a decode step, more a prompt's last window.  q [n][n_q][n_heads][R+P],
+ * lse [n][n_q][n_heads], f32, q 16-byte aligned; R = 512, P = 64, n_heads <= 32.
+ * old_lens [n] (NULL: all positions are old) marks where sums start anew, so
+ * rows appended since the last call need no zeroing.  Positions >= len are left
+ * as they were; a length beyond the table or mass_stride sets
+ * KVCU_STATUS_BAD_LEN and is cut, a bad block sets KVCU_STATUS_BAD_BLOCK and its
+ * positions are left.  Entries may share a sequence (each has its own sums).
+ * Runs on the last one-layer plan of `ws` (kvcu_decode_plan or _causal; the
+ * batch must be the one planned), so a step's decode and its mass share it. */
+int kvcu_attn_mass(kvcu_decode_ws* ws, kvcu_pool* pool, uint32_t layer, uint32_t n, const uint32_t* seq_ids,
+                   uint32_t n_seqs, const uint32_t* table_offsets, const uint32_t* tables, const uint32_t* lens,
+                   uint32_t n_q, const float* q, const float* lse, uint32_t n_heads, float scale, float decay,
+                   const uint32_t* old_lens, float* mass, uint64_t mass_stride, void* stream);
+
+/* Which positions stay, for every layer i < n_layers and entry b < n: with len =
+ * lens[seq], all of them when len <= budget; else the first n_sink, the last
+ * n_recent, and of those between the budget - n_sink - n_recent largest
+ * mass[i*mass_layer_stride + b*mass_stride + p] (equal sums: the lowest
+ * position; NaN ranks below every number).  keep[i*keep_layer_stride +
+ * b*keep_stride + j], j < budget: the positions in ascending order, then
+ * KVCU_NO_POSITION; keep_counts[b] = min(len, budget).  n_sink + n_recent <=
+ * budget <= keep_stride.  A length beyond mass_stride sets KVCU_STATUS_BAD_LEN
+ * and is cut.  `pool` gives the device and the status word. */
+#define KVCU_NO_POSITION 0xFFFFFFFFu
+int kvcu_evict_select(kvcu_pool* pool, uint32_t n_layers, uint32_t n, const uint32_t* seq_ids, uint32_t n_seqs,
+                      const uint32_t* lens, uint32_t budget, uint32_t n_sink, uint32_t n_recent, const float* mass,
+                      uint64_t mass_layer_stride, uint64_t mass_stride, uint32_t* keep, uint64_t keep_layer_stride,
+                      uint64_t keep_stride, uint32_t* keep_counts, void* stream);
+
+/* Row j of entry b's sequence := its row keep[..][j], j < keep_counts[b], in
+ * layers [layer, layer + n_layers) (keep's layer i for layer + i), in place
+ * through the block table; mass (may be NULL) moves along, mass[j] :=
+ * mass[keep[j]]; lens (may be NULL): lens[seq] := keep_counts[b].  keep must
+ * ascend strictly, and a sequence may appear once in the batch.  Rows behind
+ * the kept ones are left as they were (free them by truncating the table);
+ * blocks are written whoever else holds them, so shared blocks must be copied
+ * first (kvcu_pool_copy_block).  Entries that point
+ * outside the table or the pool set the status word and their row is left. */
+int kvcu_evict_compact(kvcu_pool* pool, uint32_t layer, uint32_t n_layers, uint32_t n, const uint32_t* seq_ids,
+                       uint32_t n_seqs, const uint32_t* table_offsets, const uint32_t* tables, const uint32_t* keep,
+                       uint64_t keep_layer_stride, uint64_t keep_stride, const uint32_t* keep_counts, float* mass,
+                       uint64_t mass_layer_stride, uint64_t mass_stride, uint32_t* lens, void* stream);
+
 /* ------------------------------------------------------------ rotary positions
  * y = m R(pos) x over the pairs of a head's rotary part: pair i is turned by
  * pos * f_i (src/math.zig:197-240 is the plain interleaved form).  A kvcu_rope

@@ -102,6 +102,12 @@ _SIGS = {
     "kvcu_decode_ws_test_withhold": (_i32, [_vp, _u32]),
     "kvcu_decode_last_impl": (_i32, [_vp]),
     "kvcu_mla_decode_noalloc": (_i32, [_vp, _u32, _u32, _vp, _u32, _vp, _vp, _vp, _vp, _u32, _f32, _vp, _vp]),
+    "kvcu_attn_mass": (_i32, [_vp, _vp, _u32, _u32, _vp, _u32, _vp, _vp, _vp, _u32, _vp, _vp, _u32, _f32, _f32, _vp,
+                              _vp, _u64, _vp]),
+    "kvcu_evict_select": (_i32, [_vp, _u32, _u32, _vp, _u32, _vp, _u32, _u32, _u32, _vp, _u64, _u64, _vp, _u64, _u64,
+                                 _vp, _vp]),
+    "kvcu_evict_compact": (_i32, [_vp, _u32, _u32, _u32, _vp, _u32, _vp, _vp, _vp, _u64, _u64, _vp, _vp, _u64, _u64,
+                                  _vp, _vp]),
     "kvcu_rope_create": (_vp, [C.POINTER(RopeDesc)]),
     "kvcu_rope_destroy": (_i32, [_vp]),
     "kvcu_rope_frequencies": (_i32, [_vp, _vp, _vp]),
@@ -229,6 +235,11 @@ def _dptr(t) -> C.c_void_p:
     return C.c_void_p(t.data_ptr())
 
 
+def _ptr(t):
+    """Device address of a torch tensor, or None."""
+    return None if t is None else t.data_ptr()
+
+
 def _stream(s) -> C.c_void_p:
     if s is None:
         return C.c_void_p(0)
@@ -325,6 +336,41 @@ class DevicePool:
                                      table_offsets.numel() - 1, _dptr(table_offsets), _dptr(tables),
                                      _dptr(out), _stream(stream)), "kvcu_gather_rows")
 
+    def evict_select(self, mass, lens, budget, n_sink, n_recent, keep, counts, seq_ids=None, stream=None):
+        """mass [n_layers][n][longest] f32 -> keep [n_layers][n][>= budget] (ascending positions, then -1)
+        and counts [n]; the first n_sink and last n_recent positions always stay."""
+        (nl, n, _), (ms, kst) = mass.shape, (mass.stride(), keep.stride())
+        if keep.shape[:2] != (nl, n) or keep.shape[2] < budget or counts.shape[0] < n or ms[2] != 1 or kst[2] != 1:
+            raise ValueError("evict_select: keep [n_layers][n][>= budget], counts [n], contiguous positions")
+        if (seq_ids.shape[0] if seq_ids is not None else lens.shape[0]) < n or (n > 1 and ms[1] != mass.shape[2]):
+            raise ValueError(f"evict_select: {n} entries in mass, fewer sequences, or rows of mass apart")
+        rc = lib().kvcu_evict_select(self._h, nl, n, _ptr(seq_ids), lens.shape[0], lens.data_ptr(), budget, n_sink,
+                                     n_recent, mass.data_ptr(), ms[0], mass.shape[2],
+                                     keep.data_ptr(), kst[0], keep.shape[2] if n == 1 else kst[1], counts.data_ptr(),
+                                     _stream(stream))
+        if rc:
+            check(rc, "kvcu_evict_select")
+
+    def evict_compact(self, layer, table_offsets, tables, keep, counts, mass=None, lens=None, seq_ids=None,
+                      stream=None):
+        """Move the kept rows (keep [n_layers][n][*], counts [n], from evict_select) of layers
+        [layer, layer + n_layers) to the front of their sequences, and mass [n_layers][n][*] with them."""
+        (nl, n, _), kst = keep.shape, keep.stride()
+        if kst[2] != 1 or (n > 1 and kst[1] != keep.shape[2]):
+            raise ValueError("evict_compact: keep [n_layers][n][positions], contiguous in a layer")
+        if mass is not None and (mass.shape[:2] != (nl, n) or mass.stride(2) != 1 or
+                                 (n > 1 and mass.stride(1) != mass.shape[2])):
+            raise ValueError("evict_compact: mass [n_layers][n][positions], contiguous in a layer")
+        n_seqs = table_offsets.shape[0] - 1
+        if (seq_ids.shape[0] if seq_ids is not None else n_seqs) < n or counts.shape[0] < n:
+            raise ValueError(f"evict_compact: {n} entries in keep, fewer sequences or counts")
+        ms = (0, 0) if mass is None else (mass.stride(0), mass.shape[2])
+        rc = lib().kvcu_evict_compact(self._h, layer, nl, n, _ptr(seq_ids), n_seqs, table_offsets.data_ptr(),
+                                      tables.data_ptr(), keep.data_ptr(), kst[0], keep.shape[2], counts.data_ptr(), _ptr(mass),
+                                      ms[0], ms[1], _ptr(lens), _stream(stream))
+        if rc:
+            check(rc, "kvcu_evict_compact")
+
     def read_checkpoint(self, offset=0, nbytes=None, stream=None) -> bytes:
         d = self.describe()
         if nbytes is None:
@@ -375,6 +421,23 @@ class DecodeWorkspace:
         check(lib().kvcu_mla_decode(self._h, pool.handle, layer, n, _dptr(seq_ids), lens.numel(),
                                     _dptr(table_offsets), _dptr(tables), _dptr(lens), _dptr(q), H,
                                     scale, _dptr(out), _stream(stream)), "kvcu_mla_decode")
+
+    def attn_mass(self, pool: DevicePool, layer, q, lse, table_offsets, tables, lens, scale, mass, decay=1.0,
+                  old_lens=None, seq_ids=None, stream=None):
+        """mass [n][longest] f32 += the attention weights of q [n][n_q][H][W] (or [n][H][W]) with the
+        log-sum-exp lse [n][n_q][H], on the last plan (kvcu_attn_mass)."""
+        n, H, W = q.shape[0], q.shape[-2], q.shape[-1]
+        n_q = q.shape[1] if q.dim() == 4 else 1
+        if not (q.is_contiguous() and lse.is_contiguous()) or lse.numel() != n * n_q * H or mass.stride(-1) != 1:
+            raise ValueError("attn_mass: contiguous q [n][n_q][H][W] and lse [n][n_q][H], mass [n][positions]")
+        if mass.shape[0] != n or (n > 1 and mass.stride(0) != mass.shape[1]) or table_offsets.shape[0] <= lens.shape[0] or (
+                old_lens is not None and old_lens.shape[0] < n):
+            raise ValueError(f"attn_mass: {n} entries in q, other sizes in mass, old_lens or table_offsets")
+        rc = lib().kvcu_attn_mass(self._h, pool.handle, layer, n, _ptr(seq_ids), lens.shape[0], table_offsets.data_ptr(),
+                                  tables.data_ptr(), lens.data_ptr(), n_q, q.data_ptr(), lse.data_ptr(), H, scale, decay,
+                                  _ptr(old_lens), mass.data_ptr(), mass.shape[1], _stream(stream))
+        if rc:
+            check(rc, "kvcu_attn_mass")
 
     def decode_layers(self, pool: DevicePool, layer, q, table_offsets, tables, lens, scale, out, seq_ids=None,
                       stream=None):
