@@ -12,6 +12,7 @@
 //
 // The scores need f32-level accuracy (an error of the score is a relative error
 // of the weight), so the products keep q's and the row's full precision.
+#include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -186,71 +187,134 @@ __global__ void __launch_bounds__(NT, 1) k_mass(MassArgs a) {
 }
 
 // ------------------------------------------------------------------ tensor cores, Q8_0 rows
-// A Q8_0 row is 18 blocks of 32 int8 values with a scale each, and int8 values are
-// exact in f16: per block, mma.sync m16n8k16 (f16, f32 accumulation) of 16 rows'
-// values against 8 columns of q, then one f32 FMA with the row's block scale.  q is
-// brought to [2^13, 2^14) by a power of two per column and slice and split into two
-// f16 parts (22 bits), so the scores have f32's accuracy at two MMAs per product;
-// rounding row or query to one f16 would cost 2e-3 of the weight.  tcgen05 does
-// not help here: its accumulators live in TMEM, and the 18 block sums of every
-// (row, column) would have to be read back from there before they can be scaled,
-// where mma.sync leaves them in the registers that scale them.
+// A Q8_0 row is 18 blocks of 32 int8 values with a scale each.  int8 values are exact
+// in f16, so per block and column D = sum of value * q runs on tcgen05 kind::f16 with
+// M = 128 rows, and one f32 FMA with the row's block scale adds D to the row's score.
+// q's columns are brought to [2^13, 2^14) by a power of two and split into two f16
+// parts (22 bits), both accumulated into D, so the scores have f32's accuracy;
+// rounding row or query to one f16 would cost 2e-3 of the weight.
 //
-// One CTA per SM, 12 compute warps and a producer.  A compute warp has 3 of the 18
-// blocks (its q parts stay in registers for a whole item) and 32 of a tile's 64
-// rows; the 6 slices' partial scores meet in shared memory, where 256 threads add
-// them, take the exponentials and sum over the columns while the other warps are
-// already in the next tile.  The producer streams rows in with bulk copies (576 B,
-// padded to 608 B in shared memory: the 8-byte fragment loads then touch every bank
-// once) through three stages, and runs ahead with the items, lengths and block
-// tables.  More than 24 columns (several queries, more heads) go in chunks: the
-// item's rows are streamed again, from L2, for each.
-constexpr int TC_WARPS = 12, TC_THREADS = (TC_WARPS + 4) * 32, SLICES = 6, BPS = 3;  // blocks per slice
-// Registers: launched with 128 a thread; the producer's four warps (three idle) give
-// theirs to the compute warps, whose q parts take 72.
-constexpr int TC_LAUNCH_REGS = 128, TC_PRODUCER_REGS = 56, TC_COMPUTE_REGS = 152;
-static_assert(TC_WARPS * TC_COMPUTE_REGS + 4 * TC_PRODUCER_REGS <= (TC_WARPS + 4) * TC_LAUNCH_REGS,
-              "register split exceeds the launch allocation");
-constexpr int TCT = 64, ROW = 608, STAGES = 3;
-constexpr uint32_t STAGE_BYTES = TCT * ROW + TCT * NBLK * 2;
-constexpr uint32_t GROUP = 16, GROUP_TX = GROUP * (W + NBLK * 2);
+// A thread owns one of a tile's 128 rows: it unpacks the row's blocks to f16 straight
+// into TMEM (the MMA's A operand), reads the block sums back from its own TMEM lane
+// and keeps the row's scores in registers.  Two warpgroups share a tile, each with
+// half of the blocks: in a step one unpacks two blocks, hands them to the issuer
+// (8 MMAs) and scales the sums of the step before, so unpacking, MMAs and scaling
+// overlap.  At the tile's end they swap halves of the columns through shared memory,
+// take the exponentials of their half, and the first adds the two sums to the mass.
+//
+//   warps 0-7   the two warpgroups
+//   warp 8      producer: TMA boxes of 128 B x <= 128 rows (a "unit": four blocks of
+//               every row of the tile; the fifth unit is the last two) through a ring
+//               of five, scales and tile descriptions through a ring of two
+//   warp 9      issues the MMAs
+//   warps 10-11 the next chunk's q parts into the other of two buffers (the first
+//               chunk is prepared by all of warps 0-7, 10, 11)
+// More columns (queries x heads) than an instance has go in chunks: the item's rows
+// are streamed again, from L2, for each.
+//
+// An earlier form on mma.sync, the sums of six slices of a row meeting in shared
+// memory, took 492 us where this one takes MASS_LARGE us (192 sequences, 2.0 M rows).
+constexpr int TC_THREADS = 384, TCT = 128, UNITS = 5;
+constexpr uint32_t UNIT_BYTES = TCT * 128;
+constexpr long long DRAIN_LIMIT = 1ll << 31;  // clocks a role that gives up waits for its own copies and MMAs
+constexpr uint32_t TM_WG = 192, TM_D = 64, TM_COLS = 512;  // TMEM columns: of a warpgroup, start of its D, allocated
+constexpr int COMPUTE = 8, PRODUCER = 8, ISSUER = 9, FILLER = 10, FILLERS = 2;
 
-struct Desc {
-  uint32_t b, p0, end, c0, old, len, ok, live;  // ok: bits of the 16-row groups; live: 0 ends the CTA's work
+enum Bar : int {
+  B_TF = 0,                // tile description and scales: full
+  B_TE = B_TF + 2,         //   read
+  B_UF = B_TE + 2,         // unit: full
+  B_UE = B_UF + UNITS,     //   read
+  B_Q0 = B_UE + UNITS,     // the first chunk's q parts
+  B_QF = B_Q0 + 1,         // q parts: full
+  B_QE = B_QF + 2,         //   done with
+  B_AF = B_QE + 2,         // unpacked blocks in TMEM, per warpgroup and buffer
+  B_DF = B_AF + 4,         // block sums ready, per warpgroup and buffer
+  B_X = B_DF + 4,          // both warpgroups' scores swapped
+  B_FINAL = B_X + 1,
+  NUM_BARS = B_FINAL + 1
 };
 
+struct Tile {
+  uint32_t b, p0, end, c0, old, ok;  // ok: bits of the boxes that were loaded
+  uint32_t chunk;                    // counts the chunks of the CTA; q buffer chunk % 2
+  uint32_t flags;                    // TILE_*
+};
+constexpr uint32_t TILE_LIVE = 1, TILE_FIRST = 2, TILE_LAST = 4;  // of its chunk
+
+template <int NC>  // columns of a chunk
+struct Map {
+  static constexpr int HC = NC / 2;
+  static constexpr int RB = (NC + 7) / 8 * 8;          // rows of a q part
+  static constexpr uint32_t N = (RB + 15) / 16 * 16;   // MMA columns: the surplus reads rows of the next part
+  static constexpr uint32_t REGION = 2 * RB * 128;     // 64 elements of the hi rows, then of the lo rows
+  static constexpr uint32_t QBUF = (W / 64) * REGION;
+  static constexpr uint32_t RING = 2 * QBUF;           // 1024-aligned, as every region and unit
+  static constexpr uint32_t SC = RING + UNITS * UNIT_BYTES;
+  static constexpr uint32_t X = SC + 2 * TCT * NBLK * 2;      // [2][warpgroup][HC][128] scores given away
+  static constexpr uint32_t S = X + 2 * 2 * HC * TCT * 4;     // [2][128] the second warpgroup's sums
+  static constexpr uint32_t COL = S + 2 * TCT * 4;            // [2][RB] scale, lse, limit
+  static constexpr uint32_t TILES = COL + 2 * RB * 12;
+  static constexpr uint32_t BARS = (TILES + 2 * sizeof(Tile) + 7) / 8 * 8;
+  static constexpr uint32_t MISC = BARS + NUM_BARS * 8;       // TMEM base, abort flag
+  static constexpr uint32_t ALLOC = MISC + 16 + 1024;
+  static_assert(ALLOC <= 232448, "shared memory budget");
+  static_assert(REGION % 1024 == 0 && NC % 4 == 0 && TM_D + 4 * N <= TM_WG, "layout");
+};
+
+struct TcMass {
+  MassArgs m;
+  uint32_t box_rows;
+  long long wait_limit;
+};
+
+// Bounded wait: false after `limit` clocks or when another role has given up.
+__device__ __forceinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, long long limit) {
+  const long long t0 = clock64();
+  while (!kvtc::mbar_try(bar, parity))
+    if (*abort_flag || clock64() - t0 > limit) {
+      *abort_flag = 1u;
+      return false;
+    }
+  return true;
+}
+// One verdict for the converged warp.
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, long long limit) {
+  const bool ok = kvtc::mbar_try(bar, parity) || wait_slow(bar, parity, abort_flag, limit);
+  return __all_sync(0xffffffffu, ok);
+}
+
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                "l"(src), "r"(bytes), "r"(bar)
                : "memory");
 }
-
-// Wait for phase `parity`, at most `limit` clocks.
-__device__ __forceinline__ bool bounded_wait(uint32_t bar, uint32_t parity, long long limit) {
-  if (kvtc::mbar_try(bar, parity)) return true;
-  const long long t0 = clock64();
-  while (!kvtc::mbar_try(bar, parity))
-    if (clock64() - t0 > limit) return false;
-  return true;
-}
-
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+// D (+)= A B with A in TMEM, f16 x f16 -> f32
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
 }
 
 // Four int8 values as two f16 pairs, exact: a biased byte u in the low mantissa of
 // 1024 is 1024 + u; minus 1152 leaves u - 128.
-__device__ __forceinline__ void int8_to_f16(uint32_t w, uint32_t* lo, uint32_t* hi) {
+__device__ __forceinline__ void int8_to_f16(uint32_t w, uint32_t* out) {
   const uint32_t u = w ^ 0x80808080u;
   const __half2 bias = __half2half2(__ushort_as_half(0x6480));
   const uint32_t x = __byte_perm(u, 0x64646464u, 0x4140), y = __byte_perm(u, 0x64646464u, 0x4342);
   const __half2 r0 = __hsub2(*reinterpret_cast<const __half2*>(&x), bias);
   const __half2 r1 = __hsub2(*reinterpret_cast<const __half2*>(&y), bias);
-  *lo = *reinterpret_cast<const uint32_t*>(&r0);
-  *hi = *reinterpret_cast<const uint32_t*>(&r1);
+  out[0] = *reinterpret_cast<const uint32_t*>(&r0);
+  out[1] = *reinterpret_cast<const uint32_t*>(&r1);
 }
 
 __device__ __forceinline__ uint32_t pack_half(float x, float y) {
@@ -258,289 +322,457 @@ __device__ __forceinline__ uint32_t pack_half(float x, float y) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-template <int NTL>  // column tiles of 8 in a chunk
-struct TcLayout {
-  static constexpr int COLS = NTL * 8;
-  static constexpr int LD = NTL == 2 ? 24 : COLS;  // floats of a row of partial scores (a stride of 16 would conflict)
-  static constexpr uint32_t RED = STAGES * STAGE_BYTES;
-  static constexpr uint32_t RED_BYTES = SLICES * TCT * LD * 4;
-  static constexpr uint32_t TOTAL = RED + 2 * RED_BYTES;
-};
-
-template <int NTL>
-__global__ void __launch_bounds__(TC_THREADS, 1) k_mass_tc(MassArgs a, long long wait_limit) {
-  using L = TcLayout<NTL>;
-  extern __shared__ __align__(128) char sm[];
-  __shared__ __align__(8) uint64_t bars[2 * STAGES];
-  __shared__ Desc descs[STAGES];
-  __shared__ uint32_t s_abort[2];
-  const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
-  const uint32_t full = kvtc::smem_u32(bars), empty = full + 8 * STAGES, base = kvtc::smem_u32(sm);
-  if (tid == 0) {
-    for (int i = 0; i < STAGES; ++i) {
-      kvtc::mbar_init(full + 8 * i, 1);
-      kvtc::mbar_init(empty + 8 * i, TC_WARPS);
-    }
-    s_abort[0] = s_abort[1] = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+// Row r of the q parts of (entry b, columns from c0), and its column's scale, lse and
+// limit; by one warp.
+template <int NC>
+__device__ __forceinline__ void fill_row(const MassArgs& a, char* sm, uint32_t buf, uint32_t r, uint32_t b, uint32_t c0,
+                                         uint32_t len, uint32_t cols, uint32_t lane) {
+  using M = Map<NC>;
+  const uint32_t c = c0 + r;
+  const bool live = r < NC && c < cols;
+  const float4* src = reinterpret_cast<const float4*>(a.q + ((uint64_t)b * cols + c) * W);
+  float4 x[5];
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < 5; ++i) {
+    const uint32_t f = lane + 32 * i;
+    x[i] = live && f < W / 4 ? src[f] : make_float4(0.f, 0.f, 0.f, 0.f);
+    amax = fmaxf(fmaxf(fmaxf(amax, fabsf(x[i].x)), fmaxf(fabsf(x[i].y), fabsf(x[i].z))), fabsf(x[i].w));
   }
-  __syncthreads();
-  const uint32_t cols = a.n_q * a.n_heads;
-
-  if (warp >= TC_WARPS) {
-    // ---------------------------------------------------------------- producer
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TC_PRODUCER_REGS));
-    if (warp > TC_WARPS) return;
-    const uint32_t n_items = a.meta[0], n_ranges = a.meta[1];
-    if (blockIdx.x == 0 && lane == 0 && n_ranges > gridDim.x) atomicOr(a.status, KVCU_STATUS_BAD_PLAN);
-    const uint32_t it0 = blockIdx.x < n_ranges ? min(a.ranges[blockIdx.x], n_items) : n_items;
-    const uint32_t it1 = blockIdx.x < n_ranges ? min(a.ranges[blockIdx.x + 1], n_items) : n_items;
-    uint32_t g = 0;  // stage uses so far
-    bool ok = true;
-    for (uint32_t base_it = it0; ok && base_it < it1; base_it += 32) {
-      // 32 items' entries at once: one chain of dependent loads for all
-      kvcu_item mine = {0, 0, 0, 0};
-      Entry me = {0, 0, 0, 0, 0};
-      if (base_it + lane < it1) {
-        mine = a.items[base_it + lane];
-        me = entry_of(a, mine.b, true);
-      }
-      const uint32_t here = min(32u, it1 - base_it);
-      for (uint32_t k = 0; ok && k < here; ++k) {
-        const uint32_t b = __shfl_sync(0xffffffffu, mine.b, k), start = __shfl_sync(0xffffffffu, mine.start, k);
-        const uint32_t len = __shfl_sync(0xffffffffu, me.len, k), old = __shfl_sync(0xffffffffu, me.old, k);
-        const uint32_t t0 = __shfl_sync(0xffffffffu, me.t0, k);
-        const uint32_t end = min(__shfl_sync(0xffffffffu, mine.end, k), len);
-        const uint32_t grp = lane >> 3;  // this lane's two rows, 2 * lane and 2 * lane + 1, lie in one 16-row group
-        auto block_at = [&](uint32_t p0) -> uint32_t {
-          const uint32_t p = p0 + grp * GROUP;
-          return p < end ? a.tables[t0 + p / a.block_size] : 0xFFFFFFFFu;
-        };
-        for (uint32_t c0 = 0; ok && c0 < cols; c0 += L::COLS) {
-          uint32_t next = block_at(start);
-          for (uint32_t p0 = start; p0 < end; p0 += TCT, ++g) {
-            const uint32_t blk = next, s = g % STAGES;
-            next = block_at(p0 + TCT < end ? p0 + TCT : end);
-            const bool in = p0 + grp * GROUP < end, good = in && blk < a.num_blocks;
-            if (in && !good && c0 == 0 && (lane & 7u) == 0) atomicOr(a.status, KVCU_STATUS_BAD_BLOCK);
-            const uint32_t votes = __ballot_sync(0xffffffffu, good && (lane & 7u) == 0);
-            ok = bounded_wait(empty + 8 * s, ((g / STAGES) & 1u) ^ 1u, wait_limit);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            const uint32_t mask = (votes & 1u) | (votes >> 7 & 2u) | (votes >> 14 & 4u) | (votes >> 21 & 8u);
-            if (lane == 0) {
-              descs[s] = {b, p0, end, c0, old, len, mask, 1u};
-              kvtc::mbar_arrive_tx(full + 8 * s, __popc(mask) * GROUP_TX);
-            }
-            __syncwarp();
-            if (good) {
-              const uint64_t row = ((uint64_t)a.layer * a.num_blocks + blk) * a.block_size + (p0 + grp * GROUP) % a.block_size;
-              const uint32_t st = base + s * STAGE_BYTES;
-              const uint32_t r = 2 * lane;
-              const int8_t* src = a.qs + (row + (r & 15u)) * W;
-              bulk_load(st + r * ROW, src, W, full + 8 * s);
-              bulk_load(st + (r + 1) * ROW, src + W, W, full + 8 * s);
-              if ((lane & 7u) == 0)
-                bulk_load(st + TCT * ROW + grp * GROUP * NBLK * 2, a.sc + row * NBLK, GROUP * NBLK * 2, full + 8 * s);
-            }
-          }
-        }
-      }
-    }
-    const uint32_t s = g % STAGES;
-    if (ok) ok = __all_sync(0xffffffffu, bounded_wait(empty + 8 * s, ((g / STAGES) & 1u) ^ 1u, wait_limit));
-    if (ok) {
-      if (lane == 0) {
-        descs[s].live = 0;
-        kvtc::mbar_arrive(full + 8 * s);
-      }
-    } else {
-      if (lane == 0) atomicOr(a.status, KVCU_STATUS_TIMEOUT);
-      // the copies in flight must land before the CTA leaves
-      for (uint32_t k = g > STAGES ? g - STAGES : 0; k < g; ++k)
-        bounded_wait(full + 8 * (k % STAGES), (k / STAGES) & 1u, wait_limit);
-    }
-    return;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  // 2^(13 - exponent of amax); 1 for a column of zeros or with an infinity
+  const uint32_t eb = __float_as_uint(amax) >> 23;
+  const uint32_t f2 = amax == 0.f || eb == 255u ? 127u : min(max(267 - (int)eb, 1), 253);
+  const float up = __uint_as_float(f2 << 23), down = __uint_as_float((254u - f2) << 23);
+  char* q = sm + buf * M::QBUF;
+#pragma unroll
+  for (int i = 0; i < 5; ++i) {
+    const uint32_t f = lane + 32 * i;  // elements 4f .. 4f + 3
+    if (f >= W / 4) continue;
+    const float y0 = x[i].x * up, y1 = x[i].y * up, y2 = x[i].z * up, y3 = x[i].w * up;
+    const uint2 hi = make_uint2(pack_half(y0, y1), pack_half(y2, y3));
+    const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&hi.x));
+    const float2 h1 = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
+    char* at = q + (f / 16) * M::REGION;
+    *reinterpret_cast<uint2*>(at + kvtc::sw128_off(r, (f % 16) * 8)) = hi;
+    *reinterpret_cast<uint2*>(at + kvtc::sw128_off(M::RB + r, (f % 16) * 8)) =
+        make_uint2(pack_half(y0 - h0.x, y1 - h0.y), pack_half(y2 - h1.x, y3 - h1.y));
   }
-
-  // ------------------------------------------------------------------ compute
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TC_COMPUTE_REGS));
-  const uint32_t slice = warp % SLICES, half = warp / SLICES;
-  const uint32_t gr = lane >> 2, t = lane & 3u;
-  uint32_t bh[BPS][2][NTL][2], bl[BPS][2][NTL][2];  // q parts: [block][k step][column tile][pair]
-  float back[NTL][2];                               // 2^-e of the columns this lane's sums belong to
-  // the adding threads: row tid / 4 of a tile, 2 * NTL columns
-  constexpr int CPT = 2 * NTL;
-  const uint32_t er = tid >> 2, ec = (tid & 3u) * CPT;
-  const bool adds = tid < 4 * TCT;
-  float lse[CPT];
-  uint32_t lim[CPT];  // positions below it count
-  float before = 0.f;
-  Desc prev = {};
-  uint32_t have_b = 0xFFFFFFFFu, have_c = 0;
-  for (uint32_t g = 0;; ++g) {
-    const uint32_t s = g % STAGES;
-    if (!bounded_wait(full + 8 * s, (g / STAGES) & 1u, wait_limit)) *(volatile uint32_t*)&s_abort[g & 1u] = 1u;
-    const Desc d = descs[s];
-    asm volatile("bar.sync 1, %0;" ::"n"(TC_WARPS * 32) : "memory");
-    // every partial score of tile g - 1 is in shared memory
-    const bool stop = *(volatile uint32_t*)&s_abort[g & 1u] != 0;
-    if (adds && prev.live) {
-      const float* red = reinterpret_cast<const float*>(sm + L::RED + ((g - 1) & 1u) * L::RED_BYTES);
-      const uint32_t p = prev.p0 + er;
-      float sc[CPT];
-#pragma unroll
-      for (int j = 0; j < CPT; ++j) sc[j] = 0.f;
-#pragma unroll
-      for (int k = 0; k < SLICES; ++k)
-#pragma unroll
-        for (int j = 0; j < CPT; j += 2) {
-          const float2 v = *reinterpret_cast<const float2*>(red + (k * TCT + er) * L::LD + ec + j);
-          sc[j] += v.x;
-          sc[j + 1] += v.y;
-        }
-      float sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < CPT; ++j)
-        if (p < lim[j]) sum += expf(fmaf(sc[j], a.scale, -lse[j]));
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      if ((tid & 3u) == 0 && p < prev.end && (prev.ok >> (er >> 4) & 1u)) {
-        float* m = a.mass + (uint64_t)prev.b * a.mass_stride + p;
-        if (prev.c0) *m = before + sum;
-        else *m = p < prev.old ? fmaf(a.decay, before, sum) : sum;
-      }
-    }
-    if (stop || !d.live) {
-      if (stop && tid == 0) atomicOr(a.status, KVCU_STATUS_TIMEOUT);
-      break;
-    }
-    if (d.b != have_b || d.c0 != have_c) {
-      have_b = d.b;
-      have_c = d.c0;
-      const float* qb = a.q + (uint64_t)d.b * cols * W;
-      float inv[NTL];
-#pragma unroll
-      for (int nt = 0; nt < NTL; ++nt) {
-        const uint32_t c = d.c0 + nt * 8 + gr;
-        float x[BPS][8];
-        float amax = 0.f;
-#pragma unroll
-        for (int i = 0; i < BPS; ++i) {
-          float4 u = make_float4(0.f, 0.f, 0.f, 0.f), v = u;
-          if (c < cols) {
-            const float4* src = reinterpret_cast<const float4*>(qb + (uint64_t)c * W + (slice * BPS + i) * 32 + t * 8);
-            u = src[0];
-            v = src[1];
-          }
-          x[i][0] = u.x, x[i][1] = u.y, x[i][2] = u.z, x[i][3] = u.w;
-          x[i][4] = v.x, x[i][5] = v.y, x[i][6] = v.z, x[i][7] = v.w;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[i][j]));
-        }
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        // 2^(13 - exponent of amax); 1 for a column of zeros or with an infinity
-        const uint32_t eb = __float_as_uint(amax) >> 23;
-        const uint32_t f = amax == 0.f || eb == 255u ? 127u : min(max(267 - (int)eb, 1), 253);
-        const float up = __uint_as_float(f << 23);
-        inv[nt] = __uint_as_float((254u - f) << 23);
-#pragma unroll
-        for (int i = 0; i < BPS; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {  // elements 2j, 2j + 1: k step j / 2, pair j % 2
-            const float y0 = x[i][2 * j] * up, y1 = x[i][2 * j + 1] * up;
-            const uint32_t h = pack_half(y0, y1);
-            const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&h));
-            bh[i][j >> 1][nt][j & 1] = h;
-            bl[i][j >> 1][nt][j & 1] = pack_half(y0 - hf.x, y1 - hf.y);
-          }
-        back[nt][0] = __shfl_sync(0xffffffffu, inv[nt], t * 8);
-        back[nt][1] = __shfl_sync(0xffffffffu, inv[nt], t * 8 + 4);
-      }
-      if (adds) {
-#pragma unroll
-        for (int j = 0; j < CPT; ++j) {
-          const uint32_t c = d.c0 + ec + j;
-          lse[j] = c < cols ? a.lse[(uint64_t)d.b * cols + c] : -INFINITY;
-          const uint32_t behind = a.n_q - 1 - c / a.n_heads;
-          // a column past the last, or a query that saw nothing, has no positions
-          lim[j] = lse[j] == -INFINITY || d.len <= behind ? 0u : d.len - behind;
-        }
-      }
-    }
-    if (adds && (tid & 3u) == 0) {
-      const uint32_t p = d.p0 + er;
-      before = p < d.end && (d.c0 || p < d.old) ? a.mass[(uint64_t)d.b * a.mass_stride + p] : 0.f;
-    }
-    const char* st = sm + s * STAGE_BYTES;
-    float* red = reinterpret_cast<float*>(sm + L::RED + (g & 1u) * L::RED_BYTES);
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      const uint32_t r0 = half * 32 + m * 16 + gr, r1 = r0 + 8;
-      float tot[NTL][4];
-#pragma unroll
-      for (int nt = 0; nt < NTL; ++nt) tot[nt][0] = tot[nt][1] = tot[nt][2] = tot[nt][3] = 0.f;
-#pragma unroll
-      for (int i = 0; i < BPS; ++i) {
-        const uint32_t blk = slice * BPS + i;
-        const uint2 w0 = *reinterpret_cast<const uint2*>(st + r0 * ROW + blk * 32 + t * 8);
-        const uint2 w1 = *reinterpret_cast<const uint2*>(st + r1 * ROW + blk * 32 + t * 8);
-        const __half* sc = reinterpret_cast<const __half*>(st + TCT * ROW);
-        const float d0 = __half2float(sc[r0 * NBLK + blk]), d1 = __half2float(sc[r1 * NBLK + blk]);
-        uint32_t af[2][4];
-        int8_to_f16(w0.x, &af[0][0], &af[0][2]);
-        int8_to_f16(w1.x, &af[0][1], &af[0][3]);
-        int8_to_f16(w0.y, &af[1][0], &af[1][2]);
-        int8_to_f16(w1.y, &af[1][1], &af[1][3]);
-#pragma unroll
-        for (int nt = 0; nt < NTL; ++nt) {
-          float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int ks = 0; ks < 2; ++ks) {
-            mma16816(acc, af[ks], bl[i][ks][nt][0], bl[i][ks][nt][1]);
-            mma16816(acc, af[ks], bh[i][ks][nt][0], bh[i][ks][nt][1]);
-          }
-          tot[nt][0] = fmaf(acc[0], d0, tot[nt][0]);
-          tot[nt][1] = fmaf(acc[1], d0, tot[nt][1]);
-          tot[nt][2] = fmaf(acc[2], d1, tot[nt][2]);
-          tot[nt][3] = fmaf(acc[3], d1, tot[nt][3]);
-        }
-      }
-#pragma unroll
-      for (int nt = 0; nt < NTL; ++nt) {
-        float* o = red + (slice * TCT + r0) * L::LD + nt * 8 + t * 2;
-        *reinterpret_cast<float2*>(o) = make_float2(tot[nt][0] * back[nt][0], tot[nt][1] * back[nt][1]);
-        *reinterpret_cast<float2*>(o + 8 * L::LD) = make_float2(tot[nt][2] * back[nt][0], tot[nt][3] * back[nt][1]);
-      }
-    }
-    __syncwarp();
-    if (lane == 0) kvtc::mbar_arrive(empty + 8 * s);
-    prev = d;
+  if (lane == 0) {
+    const float l = live ? a.lse[(uint64_t)b * cols + c] : -INFINITY;
+    const uint32_t behind = a.n_q - 1 - c / a.n_heads;  // positions behind the column's query
+    float* col = reinterpret_cast<float*>(sm + M::COL) + buf * 3 * M::RB;
+    col[r] = a.scale * down;
+    col[M::RB + r] = l;
+    // a column past the last, or a query that saw nothing, has no positions
+    reinterpret_cast<uint32_t*>(col)[2 * M::RB + r] = l == -INFINITY || len <= behind ? 0u : len - behind;
   }
 }
 
-template <int NTL>
-int launch_mass_tc(const MassArgs& a, uint32_t grid, long long wait_limit, cudaStream_t st) {
-  const int rc = kvcu_configure_once(
-      reinterpret_cast<const void*>(k_mass_tc<NTL>),
-      [](const void*) {
-        // the register split assumes exactly this many at launch: with fewer, setmaxnreg.inc would wait for ever
-        cudaFuncAttributes fa;
-        KVCU_CUDA(cudaFuncGetAttributes(&fa, k_mass_tc<NTL>));
-        if (fa.numRegs != TC_LAUNCH_REGS) {
-          kvcu_set_error("attn_mass: built with %d registers per thread, the register split needs %d", fa.numRegs,
-                         TC_LAUNCH_REGS);
-          return KVCU_ERR_UNSUPPORTED;
+// The CTA's items one after another, 32 at a time so that their chains of dependent
+// loads (item, sequence, length and table) run side by side.  All lanes of a warp.
+struct Items {
+  uint32_t it, it1, at;  // next item; end; items of the batch used
+  kvcu_item mine;
+  Entry me;
+  uint32_t b, start, end, len, old, t0;  // the current item
+  __device__ __forceinline__ bool next(const MassArgs& a, uint32_t lane, bool report) {
+    while (it < it1) {
+      const uint32_t k = at & 31u;
+      if (k == 0) {
+        mine = {0, 0, 0, 0};
+        me = {0, 0, 0, 0, 0};
+        if (it + lane < it1) {
+          mine = a.items[it + lane];
+          me = entry_of(a, mine.b, report);
         }
+      }
+      b = __shfl_sync(0xffffffffu, mine.b, k);
+      start = __shfl_sync(0xffffffffu, mine.start, k);
+      len = __shfl_sync(0xffffffffu, me.len, k);
+      old = __shfl_sync(0xffffffffu, me.old, k);
+      t0 = __shfl_sync(0xffffffffu, me.t0, k);
+      end = min(__shfl_sync(0xffffffffu, mine.end, k), len);
+      ++it;
+      ++at;
+      if (start < end) return true;
+    }
+    return false;
+  }
+};
+
+template <int NC>
+__global__ void __launch_bounds__(TC_THREADS, 1)
+    k_mass_tc(const __grid_constant__ CUtensorMap wide, const __grid_constant__ CUtensorMap tail, const TcMass t) {
+  using M = Map<NC>;
+  const MassArgs& a = t.m;
+  extern __shared__ char raw[];
+  char* sm = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t base = kvtc::smem_u32(sm);
+  const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(sm + M::MISC + 4);
+  auto bar = [&](int i) { return base + M::BARS + 8u * (uint32_t)i; };
+  auto wait = [&](int i, uint32_t parity) { return wait_bar(bar(i), parity, abort_flag, t.wait_limit); };
+  if (tid == 0) {
+    const int counts[NUM_BARS] = {1, 1, COMPUTE + 1, COMPUTE + 1, 1, 1, 1, 1, 1, COMPUTE, COMPUTE, COMPUTE, COMPUTE, COMPUTE,
+                                  COMPUTE + FILLERS, FILLERS, FILLERS, COMPUTE, COMPUTE, 4, 4, 4, 4, 1, 1, 1, 1, COMPUTE, 1};
+    for (int i = 0; i < NUM_BARS; ++i) kvtc::mbar_init(bar(i), counts[i]);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == ISSUER) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + M::MISC), "r"(TM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  kvcu_pdl_wait();  // launched programmatically: the set-up above overlaps the previous kernel's tail
+  kvtc::tc_fence_before();
+  __syncthreads();
+  kvtc::tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sm + M::MISC);
+  const uint32_t cols = a.n_q * a.n_heads;
+  const uint32_t n_items = a.meta[0], n_ranges = a.meta[1];
+  Items items = {};
+  items.it = blockIdx.x < n_ranges ? min(a.ranges[blockIdx.x], n_items) : n_items;
+  items.it1 = blockIdx.x < n_ranges ? min(a.ranges[blockIdx.x + 1], n_items) : n_items;
+  const Tile* tiles = reinterpret_cast<const Tile*>(sm + M::TILES);
+  // the q parts of chunk c of the CTA: the first has a barrier of its own
+  auto wait_q = [&](uint32_t c) { return c == 0 ? wait(B_Q0, 0) : wait(B_QF + (c & 1u), ((c >> 1) - (c & 1u ? 0 : 1)) & 1u); };
+
+  if (warp == PRODUCER) {
+    // ---------------------------------------------------------------- producer
+    if (blockIdx.x == 0 && lane == 0 && n_ranges > gridDim.x) atomicOr(a.status, KVCU_STATUS_BAD_PLAN);
+    const uint32_t boxes = TCT / t.box_rows;
+    uint32_t ti = 0, ui = 0, chunk = 0;
+    bool ok = true;
+    while (ok && items.next(a, lane, true)) {
+      auto block_at = [&](uint32_t p0) -> uint32_t {  // of this lane's box
+        const uint32_t p = p0 + lane * t.box_rows;
+        return lane < boxes && p < items.end ? a.tables[items.t0 + p / a.block_size] : 0xFFFFFFFFu;
+      };
+      for (uint32_t c0 = 0; ok && c0 < cols; c0 += NC, ++chunk) {
+        uint32_t next = block_at(items.start);
+        for (uint32_t p0 = items.start; ok && p0 < items.end; p0 += TCT, ++ti) {
+          const uint32_t blk = next, p = p0 + lane * t.box_rows;
+          next = block_at(p0 + TCT < items.end ? p0 + TCT : items.end);
+          const bool in = lane < boxes && p < items.end, good = in && blk < a.num_blocks;
+          if (in && !good && c0 == 0) atomicOr(a.status, KVCU_STATUS_BAD_BLOCK);
+          const uint32_t votes = __ballot_sync(0xffffffffu, good);
+          const uint64_t row = ((uint64_t)a.layer * a.num_blocks + blk) * a.block_size + p % a.block_size;
+          const uint32_t ts = ti & 1u;
+          if (!(ok = wait(B_TE + ts, ((ti >> 1) & 1u) ^ 1u))) break;
+          if (lane == 0) {
+            const uint32_t flags = TILE_LIVE | (p0 == items.start ? TILE_FIRST : 0u) |
+                                   (p0 + TCT >= items.end ? TILE_LAST : 0u);
+            *reinterpret_cast<Tile*>(sm + M::TILES + ts * sizeof(Tile)) = {items.b, p0, items.end, c0, items.old, votes,
+                                                                           chunk, flags};
+            kvtc::mbar_arrive_tx(bar(B_TF + ts), __popc(votes) * t.box_rows * NBLK * 2);
+          }
+          __syncwarp();
+          if (good)
+            bulk_load(base + M::SC + (ts * TCT + lane * t.box_rows) * NBLK * 2, a.sc + row * NBLK, t.box_rows * NBLK * 2,
+                      bar(B_TF + ts));
+          for (uint32_t u = 0; u < UNITS; ++u, ++ui) {
+            const uint32_t slot = ui % UNITS, width = u < 4 ? 128u : 64u;
+            if (!(ok = wait(B_UE + slot, ((ui / UNITS) & 1u) ^ 1u))) break;
+            if (lane == 0) kvtc::mbar_arrive_tx(bar(B_UF + slot), __popc(votes) * t.box_rows * width);
+            __syncwarp();
+            if (good)
+              tma_2d(base + M::RING + slot * UNIT_BYTES + lane * t.box_rows * width, u < 4 ? &wide : &tail, (int)(u * 128),
+                     (int)row, bar(B_UF + slot));
+          }
+        }
+      }
+    }
+    if (ok && (ok = wait(B_TE + (ti & 1u), ((ti >> 1) & 1u) ^ 1u)) && lane == 0) {
+      reinterpret_cast<Tile*>(sm + M::TILES)[ti & 1u].flags = 0;
+      kvtc::mbar_arrive(bar(B_TF + (ti & 1u)));
+    }
+    if (!ok) {
+      // the copies in flight must land before the CTA leaves
+      const long long t0 = clock64();
+      for (uint32_t k = ui > UNITS ? ui - UNITS : 0; k < ui; ++k)
+        while (!kvtc::mbar_try(bar(B_UF + k % UNITS), (k / UNITS) & 1u) && clock64() - t0 <= DRAIN_LIMIT) {
+        }
+      for (uint32_t k = ti > 2 ? ti - 2 : 0; k < ti; ++k)
+        while (!kvtc::mbar_try(bar(B_TF + (k & 1u)), (k >> 1) & 1u) && clock64() - t0 <= DRAIN_LIMIT) {
+        }
+    }
+  } else if (warp == ISSUER) {
+    // ---------------------------------------------------------------- MMA issuer
+    // kind::f16: D f32 (bit 4), A and B f16, both K-major, N >> 3 at bit 17, M >> 4 at bit 24
+    constexpr uint32_t IDESC = (1u << 4) | ((M::N >> 3) << 17) | ((uint32_t)(TCT >> 4) << 24);
+    uint32_t j = 0;
+    bool ok = true;
+    for (uint32_t ti = 0; ok; ++ti) {
+      if (!wait(B_TF + (ti & 1u), (ti >> 1) & 1u)) break;
+      const uint32_t flags = tiles[ti & 1u].flags, chunk = tiles[ti & 1u].chunk;
+      __syncwarp();
+      if (lane == 0) kvtc::mbar_arrive(bar(B_TE + (ti & 1u)));
+      if (!(flags & TILE_LIVE)) break;
+      if ((flags & TILE_FIRST) && !wait_q(chunk)) break;
+      const uint32_t q = base + (chunk & 1u) * M::QBUF;
+      for (uint32_t u = 0; ok && u < UNITS; ++u, ++j) {
+        const uint32_t f = j & 1u;
+        for (uint32_t g = 0; g < 2; ++g) {
+          if (!(ok = wait(B_AF + 2 * g + f, (j >> 1) & 1u))) break;
+          kvtc::tc_fence_after();
+          if (kvtc::elect_one()) {
+            const uint32_t ta = tmem + g * TM_WG + f * 32u, td = tmem + g * TM_WG + TM_D + f * 2u * M::N;
+            const uint32_t blocks = u < 4 ? 2u : 1u;
+            for (uint32_t e = 0; e < blocks; ++e) {
+              const uint32_t blk = u < 4 ? 4 * u + 2 * g + e : 16 + g;
+              const uint32_t at = q + (blk >> 1) * M::REGION + (blk & 1u) * 64u;
+#pragma unroll
+              for (uint32_t ks = 0; ks < 2; ++ks) {
+                mma_ts(td + e * M::N, ta + e * 16u + ks * 8u, kvtc::smem_desc(at + ks * 32u, 16, 1024, kvtc::LAYOUT_SW128),
+                       IDESC, ks);
+                mma_ts(td + e * M::N, ta + e * 16u + ks * 8u,
+                       kvtc::smem_desc(at + M::RB * 128u + ks * 32u, 16, 1024, kvtc::LAYOUT_SW128), IDESC, 1u);
+              }
+            }
+            kvtc::mma_commit(bar(B_DF + 2 * g + f));
+          }
+          __syncwarp();
+        }
+      }
+    }
+    // all issued MMAs retire before TMEM is freed
+    if (kvtc::elect_one()) kvtc::mma_commit(bar(B_FINAL));
+    __syncwarp();
+    const long long t0 = clock64();
+    while (!kvtc::mbar_try(bar(B_FINAL), 0) && clock64() - t0 <= DRAIN_LIMIT) {
+    }
+  } else {
+    // ---------------------------------------------------------------- the first chunk's q parts
+    const bool any = items.next(a, lane, false);
+    if (any) {
+      for (uint32_t r = warp < COMPUTE ? warp : warp - 2; r < (uint32_t)M::RB; r += COMPUTE + FILLERS)
+        fill_row<NC>(a, sm, 0, r, items.b, 0, items.len, cols, lane);
+      kvtc::fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) kvtc::mbar_arrive(bar(B_Q0));
+    }
+    if (warp >= FILLER) {
+      // -------------------------------------------------------------- the later chunks' q parts
+      uint32_t c0 = NC, chunk = 1;
+      bool ok = any;
+      while (ok) {
+        if (c0 >= cols) {
+          if (!items.next(a, lane, false)) break;
+          c0 = 0;
+        }
+        if (!(ok = wait(B_QE + (chunk & 1u), ((chunk >> 1) & 1u) ^ 1u))) break;
+        for (uint32_t r = warp - FILLER; r < (uint32_t)M::RB; r += FILLERS)
+          fill_row<NC>(a, sm, chunk & 1u, r, items.b, c0, items.len, cols, lane);
+        kvtc::fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) kvtc::mbar_arrive(bar(B_QF + (chunk & 1u)));
+        c0 += NC;
+        ++chunk;
+      }
+    } else {
+      // -------------------------------------------------------------- the warpgroups
+      constexpr int HC = M::HC;
+      const uint32_t g = warp >> 2, r = (warp & 3u) * 32u + lane;
+      const uint32_t tw = tmem + ((warp & 3u) * 32u << 16) + g * TM_WG;
+      float* xs = reinterpret_cast<float*>(sm + M::X);
+      float* sums = reinterpret_cast<float*>(sm + M::S);
+      uint32_t j = 0, ui = 0, ti = 0;
+      // the first warpgroup: the tile before, whose mass is written once the other's sum is there
+      float* out = nullptr;
+      float keep_old = 0.f, factor = 1.f, own = 0.f;
+      bool ok = true;
+      float2 tot[NC / 2];
+      auto drain = [&](uint32_t jj, int blocks, uint32_t scales) -> bool {
+        const uint32_t f = jj & 1u;
+        if (!wait(B_DF + 2 * g + f, (jj >> 1) & 1u)) return false;
+        kvtc::tc_fence_after();
+        const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&scales));
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (e < blocks) {
+            uint32_t v[NC];
+            kvtc::tmem_ld<NC>(tw + TM_D + f * 2u * M::N + e * M::N, v);
+            kvtc::tmem_wait_ld();
+            kvtc::reg_fence(v);
+            const float de = e ? d.y : d.x;
+#pragma unroll
+            for (int c = 0; c < NC / 2; ++c)
+              tot[c] = __ffma2_rn(make_float2(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1])),
+                                  make_float2(de, de), tot[c]);
+          }
+        }
+        return true;
+      };
+      while (true) {
+        const uint32_t ts = ti & 1u;
+        if (!(ok = wait(B_TF + ts, (ti >> 1) & 1u))) break;
+        const Tile d = tiles[ts];
+        uint32_t scales[5];  // of this warpgroup's blocks: pairs 2u, 2u + 1 of unit u; the last is one block
+        const uint32_t* sp = reinterpret_cast<const uint32_t*>(sm + M::SC + (ts * TCT + r) * NBLK * 2);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) scales[u] = sp[2 * u + g];
+        scales[4] = g ? sp[8] >> 16 : sp[8];
+        __syncwarp();
+        if (lane == 0) kvtc::mbar_arrive(bar(B_TE + ts));
+        if (!(d.flags & TILE_LIVE)) break;
+        if ((d.flags & TILE_FIRST) && !(ok = wait_q(d.chunk))) break;
+#pragma unroll
+        for (int c = 0; c < NC / 2; ++c) tot[c] = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u, ++ui, ++j) {
+          const uint32_t slot = ui % UNITS;
+          if (!(ok = wait(B_UF + slot, (ui / UNITS) & 1u))) break;
+          const char* st = sm + M::RING + slot * UNIT_BYTES;
+          uint32_t af[32];
+          const uint32_t ta = tw + (j & 1u) * 32u;
+          if (u < 4) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint4 w = *reinterpret_cast<const uint4*>(st + kvtc::sw128_off(r, (g * 4 + k) * 16));
+              int8_to_f16(w.x, af + 8 * k);
+              int8_to_f16(w.y, af + 8 * k + 2);
+              int8_to_f16(w.z, af + 8 * k + 4);
+              int8_to_f16(w.w, af + 8 * k + 6);
+            }
+            kvtc::tmem_st<32>(ta, af);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const uint4 w = *reinterpret_cast<const uint4*>(st + kvtc::sw64_off(r, (g * 2 + k) * 16));
+              int8_to_f16(w.x, af + 8 * k);
+              int8_to_f16(w.y, af + 8 * k + 2);
+              int8_to_f16(w.z, af + 8 * k + 4);
+              int8_to_f16(w.w, af + 8 * k + 6);
+            }
+            kvtc::tmem_st<16>(ta, af);
+          }
+          kvtc::tmem_wait_st();
+          kvtc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            kvtc::mbar_arrive(bar(B_UE + slot));
+            kvtc::mbar_arrive(bar(B_AF + 2 * g + (j & 1u)));
+          }
+          if (u > 0 && !(ok = drain(j - 1, 2, scales[u > 0 ? u - 1 : 0]))) break;
+        }
+        if (!ok || !(ok = drain(j - 1, 1, scales[4]))) break;
+        // ---- the tile's scores: each warpgroup gives away the other's half of the columns
+        float* give = xs + (ts * 2 + g) * HC * TCT + r;
+        const float* got = xs + (ts * 2 + (g ^ 1u)) * HC * TCT + r;
+        float mine[HC];
+#pragma unroll
+        for (int c = 0; c < HC; ++c) {
+          const float lo = c & 1 ? tot[c / 2].y : tot[c / 2].x;
+          const int c2 = c + HC;
+          const float hi = c2 & 1 ? tot[c2 / 2].y : tot[c2 / 2].x;
+          mine[c] = g ? hi : lo;
+          give[c * TCT] = g ? lo : hi;
+        }
+        __syncwarp();
+        if (lane == 0) kvtc::mbar_arrive(bar(B_X));
+        if (!(ok = wait(B_X, ti & 1u))) break;
+        if (out) *out = fmaf(factor, keep_old, own + sums[(ts ^ 1u) * TCT + r]);
+        const uint32_t qb = d.chunk & 1u, p = d.p0 + r;
+        const float* col = reinterpret_cast<const float*>(sm + M::COL) + qb * 3 * M::RB + g * HC;
+        float sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < HC; ++c) {
+          const float s = mine[c] + got[c * TCT];
+          if (p < reinterpret_cast<const uint32_t*>(col)[2 * M::RB + c]) sum += expf(fmaf(s, col[c], -col[M::RB + c]));
+        }
+        if (g) {
+          sums[ts * TCT + r] = sum;
+        } else {
+          own = sum;
+          out = nullptr;
+          keep_old = 0.f;
+          if (p < d.end && (d.ok >> (r / t.box_rows) & 1u)) {
+            out = a.mass + (uint64_t)d.b * a.mass_stride + p;
+            factor = d.c0 ? 1.f : a.decay;
+            if (d.c0 || p < d.old) keep_old = *out;
+          }
+        }
+        if (d.flags & TILE_LAST) {
+          __syncwarp();
+          if (lane == 0) kvtc::mbar_arrive(bar(B_QE + qb));
+        }
+        ++ti;
+      }
+      if (ok) {  // the last tile's sums
+        __syncwarp();
+        if (lane == 0) kvtc::mbar_arrive(bar(B_X));
+        if (wait(B_X, ti & 1u) && out) *out = fmaf(factor, keep_old, own + sums[((ti & 1u) ^ 1u) * TCT + r]);
+      }
+    }
+  }
+  // ---- teardown
+  kvcu_pdl_trigger();
+  __syncwarp();
+  kvtc::tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && *abort_flag) atomicOr(a.status, KVCU_STATUS_TIMEOUT);
+  if (warp == ISSUER) {
+    kvtc::tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TM_COLS) : "memory");
+  }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// Boxes of a row's 128-byte pieces (bytes 0 .. 511) and of its last 64 bytes.
+int make_maps(const kvcu_pool* p, uint32_t box_rows, CUtensorMap* wide, CUtensorMap* tail) {
+  static EncodeTiledFn enc = []() -> EncodeTiledFn {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return nullptr;
+    return reinterpret_cast<EncodeTiledFn>(f);
+  }();
+  if (!enc) {
+    kvcu_set_error("cuTensorMapEncodeTiled unavailable");
+    return KVCU_ERR_CUDA;
+  }
+  const cuuint64_t dims[2] = {(cuuint64_t)W, (cuuint64_t)p->rows()};
+  const cuuint64_t strides[1] = {(cuuint64_t)W};
+  const cuuint32_t estr[2] = {1, 1}, box_wide[2] = {128, box_rows}, box_tail[2] = {64, box_rows};
+  const CUresult r = enc(wide, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, p->qs, dims, strides, box_wide, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r2 = enc(tail, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, p->qs, dims, strides, box_tail, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS || r2 != CUDA_SUCCESS) {
+    kvcu_set_error("cuTensorMapEncodeTiled failed: %d, %d", (int)r, (int)r2);
+    return KVCU_ERR_CUDA;
+  }
+  return KVCU_OK;
+}
+
+template <int NC>
+int launch_mass_tc(const kvcu_pool* pool, const MassArgs& a, uint32_t grid, long long wait_limit, cudaStream_t st) {
+  const int rc = kvcu_configure_once(
+      reinterpret_cast<const void*>(k_mass_tc<NC>),
+      [](const void*) {
         return kvcu_check_cuda(
-            cudaFuncSetAttribute(k_mass_tc<NTL>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcLayout<NTL>::TOTAL),
+            cudaFuncSetAttribute(k_mass_tc<NC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Map<NC>::ALLOC),
             "cudaFuncSetAttribute(mass)");
       },
       nullptr);
   if (rc) return rc;
-  k_mass_tc<NTL><<<grid, TC_THREADS, TcLayout<NTL>::TOTAL, st>>>(a, wait_limit);
-  return kvcu_check_cuda(cudaGetLastError(), "attention mass launch");
+  TcMass t = {a, 128, wait_limit};
+  while (pool->block_size % t.box_rows) t.box_rows /= 2;  // block sizes are multiples of 16
+  CUtensorMap wide, tail;
+  const int rm = make_maps(pool, t.box_rows, &wide, &tail);
+  if (rm) return rm;
+  return kvcu_check_cuda(
+      kvcu_launch_pdl(k_mass_tc<NC>, dim3(grid), dim3(TC_THREADS), Map<NC>::ALLOC, st, wide, tail, t),
+      "attention mass launch");
 }
 
 int launch_mass(const MassArgs& a, uint32_t grid, cudaStream_t st) {
@@ -636,13 +868,17 @@ extern "C" int kvcu_attn_mass(kvcu_decode_ws* ws, kvcu_pool* pool, uint32_t laye
   const cudaStream_t st = (cudaStream_t)stream;
   const uint32_t grid = (uint32_t)ws->decode_ctas;
   if (!pool->quantized) return launch_mass(a, grid, st);
+  if (pool->rows() > 0x7FFFFFFFull) {
+    kvcu_set_error("kvcu_attn_mass: %llu rows, TMA coordinates reach 2^31 - 1", (unsigned long long)pool->rows());
+    return KVCU_ERR_UNSUPPORTED;
+  }
   const long long limit = ws->wait_limit ? (long long)ws->wait_limit : (1ll << 31);
-  // column tiles per chunk: a chunk costs its tiles and, whatever their number, the
-  // rows' unpacking (about three half tiles)
+  // columns of a chunk: a chunk costs its columns' scaling and exponentials and,
+  // whatever their number, the rows' unpacking (as much as about 30 columns)
   const uint32_t cols = n_q * n_heads;
-  auto cost = [&](uint32_t nt) { return ((cols + 8 * nt - 1) / (8 * nt)) * (2 * nt + 3); };
-  const uint32_t nt = cost(1) <= cost(2) && cost(1) <= cost(3) ? 1u : cost(2) <= cost(3) ? 2u : 3u;
-  if (nt == 1) return launch_mass_tc<1>(a, grid, limit, st);
-  if (nt == 2) return launch_mass_tc<2>(a, grid, limit, st);
-  return launch_mass_tc<3>(a, grid, limit, st);
+  auto cost = [&](uint32_t nc) { return (uint64_t)((cols + nc - 1) / nc) * (nc + 30); };
+  if (cost(8) <= cost(16) && cost(8) <= cost(20) && cost(8) <= cost(24)) return launch_mass_tc<8>(pool, a, grid, limit, st);
+  if (cost(16) <= cost(20) && cost(16) <= cost(24)) return launch_mass_tc<16>(pool, a, grid, limit, st);
+  if (cost(20) <= cost(24)) return launch_mass_tc<20>(pool, a, grid, limit, st);
+  return launch_mass_tc<24>(pool, a, grid, limit, st);
 }
