@@ -206,9 +206,9 @@ __global__ void __launch_bounds__(NT, 1) k_mass(MassArgs a) {
 //   warp 8      producer: TMA boxes of 128 B x <= 128 rows (a "unit": four blocks of
 //               every row of the tile; the fifth unit is the last two) through a ring
 //               of five, scales and tile descriptions through a ring of two
-//   warp 9      issues the MMAs
-//   warps 10-11 the next chunk's q parts into the other of two buffers (the first
-//               chunk is prepared by all of warps 0-7, 10, 11)
+//   warps 9-10  issue the MMAs, one for each warpgroup
+//   warp 11     the next chunk's q parts into the other of two buffers (the first
+//               chunk is prepared by all warps but the producer)
 // More columns (queries x heads) than an instance has go in chunks: the item's rows
 // are streamed again, from L2, for each.
 //
@@ -218,7 +218,7 @@ constexpr int TC_THREADS = 384, TCT = 128, UNITS = 5;
 constexpr uint32_t UNIT_BYTES = TCT * 128;
 constexpr long long DRAIN_LIMIT = 1ll << 31;  // clocks a role that gives up waits for its own copies and MMAs
 constexpr uint32_t TM_WG = 192, TM_D = 64, TM_COLS = 512;  // TMEM columns: of a warpgroup, start of its D, allocated
-constexpr int COMPUTE = 8, PRODUCER = 8, ISSUER = 9, FILLER = 10, FILLERS = 2;
+constexpr int COMPUTE = 8, PRODUCER = 8, ISSUER = 9 /* two */, FILLER = 11;
 
 enum Bar : int {
   B_TF = 0,                // tile description and scales: full
@@ -231,8 +231,8 @@ enum Bar : int {
   B_AF = B_QE + 2,         // unpacked blocks in TMEM, per warpgroup and buffer
   B_DF = B_AF + 4,         // block sums ready, per warpgroup and buffer
   B_X = B_DF + 4,          // both warpgroups' scores swapped
-  B_FINAL = B_X + 1,
-  NUM_BARS = B_FINAL + 1
+  B_FINAL = B_X + 1,       // all MMAs of an issuer retired
+  NUM_BARS = B_FINAL + 2
 };
 
 struct Tile {
@@ -322,52 +322,69 @@ __device__ __forceinline__ uint32_t pack_half(float x, float y) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Row r of the q parts of (entry b, columns from c0), and its column's scale, lse and
-// limit; by one warp.
+// Rows first, first + step, ... of the q parts of (entry b, columns from c0) and their
+// columns' scales, by one warp; the next row is loaded while one is split.
 template <int NC>
-__device__ __forceinline__ void fill_row(const MassArgs& a, char* sm, uint32_t buf, uint32_t r, uint32_t b, uint32_t c0,
-                                         uint32_t len, uint32_t cols, uint32_t lane) {
+__device__ __forceinline__ void fill_rows(const MassArgs& a, char* sm, uint32_t buf, uint32_t first, uint32_t step,
+                                          uint32_t b, uint32_t c0, uint32_t cols, uint32_t lane) {
   using M = Map<NC>;
-  const uint32_t c = c0 + r;
-  const bool live = r < NC && c < cols;
-  const float4* src = reinterpret_cast<const float4*>(a.q + ((uint64_t)b * cols + c) * W);
-  float4 x[5];
-  float amax = 0.f;
-#pragma unroll
-  for (int i = 0; i < 5; ++i) {
-    const uint32_t f = lane + 32 * i;
-    x[i] = live && f < W / 4 ? src[f] : make_float4(0.f, 0.f, 0.f, 0.f);
-    amax = fmaxf(fmaxf(fmaxf(amax, fabsf(x[i].x)), fmaxf(fabsf(x[i].y), fabsf(x[i].z))), fabsf(x[i].w));
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  // 2^(13 - exponent of amax); 1 for a column of zeros or with an infinity
-  const uint32_t eb = __float_as_uint(amax) >> 23;
-  const uint32_t f2 = amax == 0.f || eb == 255u ? 127u : min(max(267 - (int)eb, 1), 253);
-  const float up = __uint_as_float(f2 << 23), down = __uint_as_float((254u - f2) << 23);
+  float* col = reinterpret_cast<float*>(sm + M::COL) + buf * 3 * M::RB;
   char* q = sm + buf * M::QBUF;
+  float4 x[5], nx[5];
+  auto load = [&](uint32_t r, float4* v) {
+    const bool live = r < NC && c0 + r < cols;
+    const float4* src = reinterpret_cast<const float4*>(a.q + ((uint64_t)b * cols + c0 + r) * W);
 #pragma unroll
-  for (int i = 0; i < 5; ++i) {
-    const uint32_t f = lane + 32 * i;  // elements 4f .. 4f + 3
-    if (f >= W / 4) continue;
-    const float y0 = x[i].x * up, y1 = x[i].y * up, y2 = x[i].z * up, y3 = x[i].w * up;
-    const uint2 hi = make_uint2(pack_half(y0, y1), pack_half(y2, y3));
-    const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&hi.x));
-    const float2 h1 = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
-    char* at = q + (f / 16) * M::REGION;
-    *reinterpret_cast<uint2*>(at + kvtc::sw128_off(r, (f % 16) * 8)) = hi;
-    *reinterpret_cast<uint2*>(at + kvtc::sw128_off(M::RB + r, (f % 16) * 8)) =
-        make_uint2(pack_half(y0 - h0.x, y1 - h0.y), pack_half(y2 - h1.x, y3 - h1.y));
+    for (int i = 0; i < 5; ++i) {
+      const uint32_t f = lane + 32 * i;
+      v[i] = live && f < W / 4 ? src[f] : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  };
+  load(first, nx);
+  for (uint32_t r = first; r < (uint32_t)M::RB; r += step) {
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 5; ++i) {
+      x[i] = nx[i];
+      amax = fmaxf(fmaxf(fmaxf(amax, fabsf(x[i].x)), fmaxf(fabsf(x[i].y), fabsf(x[i].z))), fabsf(x[i].w));
+    }
+    if (r + step < (uint32_t)M::RB) load(r + step, nx);
+    // all values are >= 0: their bits order as integers
+    const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(amax));
+    // 2^(13 - exponent of the maximum); 1 for a column of zeros or with an infinity
+    const uint32_t eb = top >> 23;
+    const uint32_t f2 = top == 0u || eb == 255u ? 127u : min(max(267 - (int)eb, 1), 253);
+    const float up = __uint_as_float(f2 << 23);
+    if (lane == 0) col[r] = a.scale * __uint_as_float((254u - f2) << 23);
+#pragma unroll
+    for (int i = 0; i < 5; ++i) {
+      const uint32_t f = lane + 32 * i;  // elements 4f .. 4f + 3
+      if (f >= W / 4) continue;
+      const float y0 = x[i].x * up, y1 = x[i].y * up, y2 = x[i].z * up, y3 = x[i].w * up;
+      const uint2 hi = make_uint2(pack_half(y0, y1), pack_half(y2, y3));
+      const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&hi.x));
+      const float2 h1 = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
+      char* at = q + (f / 16) * M::REGION;
+      *reinterpret_cast<uint2*>(at + kvtc::sw128_off(r, (f % 16) * 8)) = hi;
+      *reinterpret_cast<uint2*>(at + kvtc::sw128_off(M::RB + r, (f % 16) * 8)) =
+          make_uint2(pack_half(y0 - h0.x, y1 - h0.y), pack_half(y2 - h1.x, y3 - h1.y));
+    }
   }
-  if (lane == 0) {
-    const float l = live ? a.lse[(uint64_t)b * cols + c] : -INFINITY;
-    const uint32_t behind = a.n_q - 1 - c / a.n_heads;  // positions behind the column's query
-    float* col = reinterpret_cast<float*>(sm + M::COL) + buf * 3 * M::RB;
-    col[r] = a.scale * down;
-    col[M::RB + r] = l;
-    // a column past the last, or a query that saw nothing, has no positions
-    reinterpret_cast<uint32_t*>(col)[2 * M::RB + r] = l == -INFINITY || len <= behind ? 0u : len - behind;
-  }
+}
+
+// Each column's lse and the positions below which it counts, a lane each.
+template <int NC>
+__device__ __forceinline__ void fill_columns(const MassArgs& a, char* sm, uint32_t buf, uint32_t b, uint32_t c0,
+                                             uint32_t len, uint32_t cols, uint32_t lane) {
+  using M = Map<NC>;
+  const uint32_t c = c0 + lane;
+  if (lane >= (uint32_t)M::RB) return;
+  const float l = lane < NC && c < cols ? a.lse[(uint64_t)b * cols + c] : -INFINITY;
+  const uint32_t behind = a.n_q - 1 - c / a.n_heads;  // positions behind the column's query
+  float* col = reinterpret_cast<float*>(sm + M::COL) + buf * 3 * M::RB;
+  col[M::RB + lane] = l;
+  // a column past the last, or a query that saw nothing, has no positions
+  reinterpret_cast<uint32_t*>(col)[2 * M::RB + lane] = l == -INFINITY || len <= behind ? 0u : len - behind;
 }
 
 // The CTA's items one after another, 32 at a time so that their chains of dependent
@@ -415,8 +432,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   auto bar = [&](int i) { return base + M::BARS + 8u * (uint32_t)i; };
   auto wait = [&](int i, uint32_t parity) { return wait_bar(bar(i), parity, abort_flag, t.wait_limit); };
   if (tid == 0) {
-    const int counts[NUM_BARS] = {1, 1, COMPUTE + 1, COMPUTE + 1, 1, 1, 1, 1, 1, COMPUTE, COMPUTE, COMPUTE, COMPUTE, COMPUTE,
-                                  COMPUTE + FILLERS, FILLERS, FILLERS, COMPUTE, COMPUTE, 4, 4, 4, 4, 1, 1, 1, 1, COMPUTE, 1};
+    const int counts[NUM_BARS] = {1, 1, COMPUTE + 2, COMPUTE + 2, 1, 1, 1, 1, 1, COMPUTE, COMPUTE, COMPUTE, COMPUTE, COMPUTE,
+                                  COMPUTE + 3, 1, 1, COMPUTE, COMPUTE, 4, 4, 4, 4, 1, 1, 1, 1, COMPUTE, 1, 1};
     for (int i = 0; i < NUM_BARS; ++i) kvtc::mbar_init(bar(i), counts[i]);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -499,62 +516,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         while (!kvtc::mbar_try(bar(B_TF + (k & 1u)), (k >> 1) & 1u) && clock64() - t0 <= DRAIN_LIMIT) {
         }
     }
-  } else if (warp == ISSUER) {
-    // ---------------------------------------------------------------- MMA issuer
-    // kind::f16: D f32 (bit 4), A and B f16, both K-major, N >> 3 at bit 17, M >> 4 at bit 24
-    constexpr uint32_t IDESC = (1u << 4) | ((M::N >> 3) << 17) | ((uint32_t)(TCT >> 4) << 24);
-    uint32_t j = 0;
-    bool ok = true;
-    for (uint32_t ti = 0; ok; ++ti) {
-      if (!wait(B_TF + (ti & 1u), (ti >> 1) & 1u)) break;
-      const uint32_t flags = tiles[ti & 1u].flags, chunk = tiles[ti & 1u].chunk;
-      __syncwarp();
-      if (lane == 0) kvtc::mbar_arrive(bar(B_TE + (ti & 1u)));
-      if (!(flags & TILE_LIVE)) break;
-      if ((flags & TILE_FIRST) && !wait_q(chunk)) break;
-      const uint32_t q = base + (chunk & 1u) * M::QBUF;
-      for (uint32_t u = 0; ok && u < UNITS; ++u, ++j) {
-        const uint32_t f = j & 1u;
-        for (uint32_t g = 0; g < 2; ++g) {
-          if (!(ok = wait(B_AF + 2 * g + f, (j >> 1) & 1u))) break;
-          kvtc::tc_fence_after();
-          if (kvtc::elect_one()) {
-            const uint32_t ta = tmem + g * TM_WG + f * 32u, td = tmem + g * TM_WG + TM_D + f * 2u * M::N;
-            const uint32_t blocks = u < 4 ? 2u : 1u;
-            for (uint32_t e = 0; e < blocks; ++e) {
-              const uint32_t blk = u < 4 ? 4 * u + 2 * g + e : 16 + g;
-              const uint32_t at = q + (blk >> 1) * M::REGION + (blk & 1u) * 64u;
-#pragma unroll
-              for (uint32_t ks = 0; ks < 2; ++ks) {
-                mma_ts(td + e * M::N, ta + e * 16u + ks * 8u, kvtc::smem_desc(at + ks * 32u, 16, 1024, kvtc::LAYOUT_SW128),
-                       IDESC, ks);
-                mma_ts(td + e * M::N, ta + e * 16u + ks * 8u,
-                       kvtc::smem_desc(at + M::RB * 128u + ks * 32u, 16, 1024, kvtc::LAYOUT_SW128), IDESC, 1u);
-              }
-            }
-            kvtc::mma_commit(bar(B_DF + 2 * g + f));
-          }
-          __syncwarp();
-        }
-      }
-    }
-    // all issued MMAs retire before TMEM is freed
-    if (kvtc::elect_one()) kvtc::mma_commit(bar(B_FINAL));
-    __syncwarp();
-    const long long t0 = clock64();
-    while (!kvtc::mbar_try(bar(B_FINAL), 0) && clock64() - t0 <= DRAIN_LIMIT) {
-    }
   } else {
     // ---------------------------------------------------------------- the first chunk's q parts
     const bool any = items.next(a, lane, false);
     if (any) {
-      for (uint32_t r = warp < COMPUTE ? warp : warp - 2; r < (uint32_t)M::RB; r += COMPUTE + FILLERS)
-        fill_row<NC>(a, sm, 0, r, items.b, 0, items.len, cols, lane);
+      const uint32_t me = warp < COMPUTE ? warp : warp - 1;
+      if (me == 0) fill_columns<NC>(a, sm, 0, items.b, 0, items.len, cols, lane);
+      fill_rows<NC>(a, sm, 0, me, COMPUTE + 3, items.b, 0, cols, lane);
       kvtc::fence_proxy_async();
       __syncwarp();
       if (lane == 0) kvtc::mbar_arrive(bar(B_Q0));
     }
-    if (warp >= FILLER) {
+    if (warp == FILLER) {
       // -------------------------------------------------------------- the later chunks' q parts
       uint32_t c0 = NC, chunk = 1;
       bool ok = any;
@@ -564,13 +537,56 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           c0 = 0;
         }
         if (!(ok = wait(B_QE + (chunk & 1u), ((chunk >> 1) & 1u) ^ 1u))) break;
-        for (uint32_t r = warp - FILLER; r < (uint32_t)M::RB; r += FILLERS)
-          fill_row<NC>(a, sm, chunk & 1u, r, items.b, c0, items.len, cols, lane);
+        fill_columns<NC>(a, sm, chunk & 1u, items.b, c0, items.len, cols, lane);
+        fill_rows<NC>(a, sm, chunk & 1u, 0, 1, items.b, c0, cols, lane);
         kvtc::fence_proxy_async();
         __syncwarp();
         if (lane == 0) kvtc::mbar_arrive(bar(B_QF + (chunk & 1u)));
         c0 += NC;
         ++chunk;
+      }
+    } else if (warp >= ISSUER) {
+      // -------------------------------------------------------------- MMA issuers, one per warpgroup
+      // kind::f16: D f32 (bit 4), A and B f16, both K-major, N >> 3 at bit 17, M >> 4 at bit 24
+      constexpr uint32_t IDESC = (1u << 4) | ((M::N >> 3) << 17) | ((uint32_t)(TCT >> 4) << 24);
+      const uint32_t g = warp - ISSUER;
+      uint32_t j = 0;
+      bool ok = true;
+      for (uint32_t ti = 0; ok; ++ti) {
+        if (!wait(B_TF + (ti & 1u), (ti >> 1) & 1u)) break;
+        const uint32_t flags = tiles[ti & 1u].flags, chunk = tiles[ti & 1u].chunk;
+        __syncwarp();
+        if (lane == 0) kvtc::mbar_arrive(bar(B_TE + (ti & 1u)));
+        if (!(flags & TILE_LIVE)) break;
+        if ((flags & TILE_FIRST) && !wait_q(chunk)) break;
+        // a descriptor's address field counts 16 bytes: offsets are added to the buffer's
+        const uint64_t q = kvtc::smem_desc(base + (chunk & 1u) * M::QBUF, 16, 1024, kvtc::LAYOUT_SW128);
+#pragma unroll
+        for (uint32_t u = 0; u < UNITS; ++u, ++j) {
+          const uint32_t f = j & 1u;
+          if (!(ok = wait(B_AF + 2 * g + f, (j >> 1) & 1u))) break;
+          kvtc::tc_fence_after();
+          if (kvtc::elect_one()) {
+            const uint32_t ta = tmem + g * TM_WG + f * 32u, td = tmem + g * TM_WG + TM_D + f * 2u * M::N;
+            // block 4u + 2g + e, the last 16 + g; two blocks to a region of 64 elements
+            const uint64_t at = q + (u < 4 ? (2 * u + g) * M::REGION : 8 * M::REGION + g * 64u) / 16;
+#pragma unroll
+            for (uint32_t e = 0; e < (u < 4 ? 2u : 1u); ++e)
+#pragma unroll
+              for (uint32_t ks = 0; ks < 2; ++ks) {
+                mma_ts(td + e * M::N, ta + e * 16u + ks * 8u, at + (e * 64u + ks * 32u) / 16, IDESC, ks);
+                mma_ts(td + e * M::N, ta + e * 16u + ks * 8u, at + (M::RB * 128u + e * 64u + ks * 32u) / 16, IDESC, 1u);
+              }
+            kvtc::mma_commit(bar(B_DF + 2 * g + f));
+          }
+          __syncwarp();
+        }
+      }
+      // all issued MMAs retire before TMEM is freed
+      if (kvtc::elect_one()) kvtc::mma_commit(bar(B_FINAL + g));
+      __syncwarp();
+      const long long t0 = clock64();
+      while (!kvtc::mbar_try(bar(B_FINAL + g), 0) && clock64() - t0 <= DRAIN_LIMIT) {
       }
     } else {
       // -------------------------------------------------------------- the warpgroups
@@ -585,11 +601,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       float keep_old = 0.f, factor = 1.f, own = 0.f;
       bool ok = true;
       float2 tot[NC / 2];
+      Tile d = {};        // the tile whose scores are being formed
+      uint32_t last = 0;  // its last block's scale
+#pragma unroll
+      for (int c = 0; c < NC / 2; ++c) tot[c] = make_float2(0.f, 0.f);
+      // adds the sums of step jj (`blocks` of them) to the scores
       auto drain = [&](uint32_t jj, int blocks, uint32_t scales) -> bool {
         const uint32_t f = jj & 1u;
         if (!wait(B_DF + 2 * g + f, (jj >> 1) & 1u)) return false;
         kvtc::tc_fence_after();
-        const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&scales));
+        const float2 sc = __half22float2(*reinterpret_cast<const __half2*>(&scales));
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           if (e < blocks) {
@@ -597,7 +618,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             kvtc::tmem_ld<NC>(tw + TM_D + f * 2u * M::N + e * M::N, v);
             kvtc::tmem_wait_ld();
             kvtc::reg_fence(v);
-            const float de = e ? d.y : d.x;
+            const float de = e ? sc.y : sc.x;
 #pragma unroll
             for (int c = 0; c < NC / 2; ++c)
               tot[c] = __ffma2_rn(make_float2(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1])),
@@ -606,10 +627,59 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         }
         return true;
       };
+      // tile d, number k of the CTA, whose last step is j1: the rest of its scores, their weights, its sums
+      auto finish = [&](uint32_t k, uint32_t j1) -> bool {
+        if (!drain(j1, 1, last)) return false;
+        if ((d.flags & TILE_FIRST) && !wait_q(d.chunk)) return false;  // its columns' scales
+        // each warpgroup gives away the other's half of the columns
+        const uint32_t ts = k & 1u;
+        float* give = xs + (ts * 2 + g) * HC * TCT + r;
+        const float* got = xs + (ts * 2 + (g ^ 1u)) * HC * TCT + r;
+        float mine[HC];
+#pragma unroll
+        for (int c = 0; c < HC; ++c) {
+          const float lo = c & 1 ? tot[c / 2].y : tot[c / 2].x;
+          const int c2 = c + HC;
+          const float hi = c2 & 1 ? tot[c2 / 2].y : tot[c2 / 2].x;
+          mine[c] = g ? hi : lo;
+          give[c * TCT] = g ? lo : hi;
+        }
+        __syncwarp();
+        if (lane == 0) kvtc::mbar_arrive(bar(B_X));
+        if (!wait(B_X, k & 1u)) return false;
+        if (out) *out = fmaf(factor, keep_old, own + sums[(ts ^ 1u) * TCT + r]);
+        const uint32_t qb = d.chunk & 1u, p = d.p0 + r;
+        const float* col = reinterpret_cast<const float*>(sm + M::COL) + qb * 3 * M::RB + g * HC;
+        float sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < HC; ++c) {
+          const float s = mine[c] + got[c * TCT];
+          if (p < reinterpret_cast<const uint32_t*>(col)[2 * M::RB + c]) sum += expf(fmaf(s, col[c], -col[M::RB + c]));
+        }
+        if (g) {
+          sums[ts * TCT + r] = sum;
+        } else {
+          own = sum;
+          out = nullptr;
+          keep_old = 0.f;
+          if (p < d.end && (d.ok >> (r / t.box_rows) & 1u)) {
+            out = a.mass + (uint64_t)d.b * a.mass_stride + p;
+            factor = d.c0 ? 1.f : a.decay;
+            if (d.c0 || p < d.old) keep_old = *out;
+          }
+        }
+        if (d.flags & TILE_LAST) {
+          __syncwarp();
+          if (lane == 0) kvtc::mbar_arrive(bar(B_QE + qb));
+        }
+#pragma unroll
+        for (int c = 0; c < NC / 2; ++c) tot[c] = make_float2(0.f, 0.f);
+        return true;
+      };
       while (true) {
         const uint32_t ts = ti & 1u;
         if (!(ok = wait(B_TF + ts, (ti >> 1) & 1u))) break;
-        const Tile d = tiles[ts];
+        const Tile now = tiles[ts];
         uint32_t scales[5];  // of this warpgroup's blocks: pairs 2u, 2u + 1 of unit u; the last is one block
         const uint32_t* sp = reinterpret_cast<const uint32_t*>(sm + M::SC + (ts * TCT + r) * NBLK * 2);
 #pragma unroll
@@ -617,10 +687,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         scales[4] = g ? sp[8] >> 16 : sp[8];
         __syncwarp();
         if (lane == 0) kvtc::mbar_arrive(bar(B_TE + ts));
-        if (!(d.flags & TILE_LIVE)) break;
-        if ((d.flags & TILE_FIRST) && !(ok = wait_q(d.chunk))) break;
-#pragma unroll
-        for (int c = 0; c < NC / 2; ++c) tot[c] = make_float2(0.f, 0.f);
+        if (!(now.flags & TILE_LIVE)) break;
 #pragma unroll
         for (int u = 0; u < UNITS; ++u, ++ui, ++j) {
           const uint32_t slot = ui % UNITS;
@@ -656,51 +723,20 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             kvtc::mbar_arrive(bar(B_UE + slot));
             kvtc::mbar_arrive(bar(B_AF + 2 * g + (j & 1u)));
           }
-          if (u > 0 && !(ok = drain(j - 1, 2, scales[u > 0 ? u - 1 : 0]))) break;
-        }
-        if (!ok || !(ok = drain(j - 1, 1, scales[4]))) break;
-        // ---- the tile's scores: each warpgroup gives away the other's half of the columns
-        float* give = xs + (ts * 2 + g) * HC * TCT + r;
-        const float* got = xs + (ts * 2 + (g ^ 1u)) * HC * TCT + r;
-        float mine[HC];
-#pragma unroll
-        for (int c = 0; c < HC; ++c) {
-          const float lo = c & 1 ? tot[c / 2].y : tot[c / 2].x;
-          const int c2 = c + HC;
-          const float hi = c2 & 1 ? tot[c2 / 2].y : tot[c2 / 2].x;
-          mine[c] = g ? hi : lo;
-          give[c * TCT] = g ? lo : hi;
-        }
-        __syncwarp();
-        if (lane == 0) kvtc::mbar_arrive(bar(B_X));
-        if (!(ok = wait(B_X, ti & 1u))) break;
-        if (out) *out = fmaf(factor, keep_old, own + sums[(ts ^ 1u) * TCT + r]);
-        const uint32_t qb = d.chunk & 1u, p = d.p0 + r;
-        const float* col = reinterpret_cast<const float*>(sm + M::COL) + qb * 3 * M::RB + g * HC;
-        float sum = 0.f;
-#pragma unroll
-        for (int c = 0; c < HC; ++c) {
-          const float s = mine[c] + got[c * TCT];
-          if (p < reinterpret_cast<const uint32_t*>(col)[2 * M::RB + c]) sum += expf(fmaf(s, col[c], -col[M::RB + c]));
-        }
-        if (g) {
-          sums[ts * TCT + r] = sum;
-        } else {
-          own = sum;
-          out = nullptr;
-          keep_old = 0.f;
-          if (p < d.end && (d.ok >> (r / t.box_rows) & 1u)) {
-            out = a.mass + (uint64_t)d.b * a.mass_stride + p;
-            factor = d.c0 ? 1.f : a.decay;
-            if (d.c0 || p < d.old) keep_old = *out;
+          // the step before: of this tile, or the last of the tile before, which is then finished
+          // while this tile's first MMAs run
+          if (u > 0) ok = drain(j - 1, 2, scales[u > 0 ? u - 1 : 0]);
+          else if (ti > 0) ok = finish(ti - 1, j - 1);
+          if (!ok) break;
+          if (u == 0) {
+            d = now;
+            last = scales[4];
           }
         }
-        if (d.flags & TILE_LAST) {
-          __syncwarp();
-          if (lane == 0) kvtc::mbar_arrive(bar(B_QE + qb));
-        }
+        if (!ok) break;
         ++ti;
       }
+      if (ok && ti > 0) ok = finish(ti - 1, j - 1);
       if (ok) {  // the last tile's sums
         __syncwarp();
         if (lane == 0) kvtc::mbar_arrive(bar(B_X));
