@@ -143,7 +143,7 @@ struct Map {
   static constexpr uint32_t SC = RING + SLOTS * UNIT_BYTES;
   static constexpr uint32_t X = SC + (Q8 ? TILE * NBLK * 2 : 0);  // [pair][warpgroup][HC][128] scores given away
   static constexpr uint32_t S = X + 2 * 2 * HC * HALF * 4;            // [pair][2][128] the second warpgroup's sums
-  static constexpr uint32_t COL = S + 2 * 2 * HALF * 4;               // [RB] scale, lse, limit
+  static constexpr uint32_t COL = S + 2 * 2 * HALF * 4;               // [RB] (scale, -lse), then limits
   static constexpr uint32_t TILES = COL + RB * 12;
   static constexpr uint32_t BARS = (TILES + sizeof(Tile) + 7) / 8 * 8;
   // barriers
@@ -171,20 +171,28 @@ struct TcMass {
   long long wait_limit;
 };
 
-// Bounded wait: false after `limit` clocks or when another role has given up.
-__device__ __forceinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, long long limit) {
+// Whether the phase is over, for the converged warp: all lanes or none.
+__device__ __forceinline__ bool try_all(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n"
+      " vote.sync.all.pred p, p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Bounded wait of the converged warp: false after `limit` clocks or when another
+// role has given up.
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, long long limit) {
+  if (try_all(bar, parity)) return true;
   const long long t0 = clock64();
-  while (!kvtc::mbar_try(bar, parity))
-    if (*abort_flag || clock64() - t0 > limit) {
+  while (!try_all(bar, parity))
+    if (__any_sync(0xffffffffu, *abort_flag || clock64() - t0 > limit)) {
       *abort_flag = 1u;
       return false;
     }
   return true;
-}
-// One verdict for the converged warp.
-__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, long long limit) {
-  const bool ok = kvtc::mbar_try(bar, parity) || wait_slow(bar, parity, abort_flag, limit);
-  return __all_sync(0xffffffffu, ok);
 }
 
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
@@ -206,6 +214,13 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
       "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+
+// 2^x by the hardware (PTX ex2.approx.f32: relative error below 2^-22).
+__device__ __forceinline__ float exp2_approx(float x) {
+  float r;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
 // Four int8 values as two f16 pairs, exact: a biased byte u in the low mantissa of
@@ -238,7 +253,7 @@ __device__ __forceinline__ uint32_t scale_field(uint32_t top) {
   return top == 0u || eb >= 255u ? 127u : (uint32_t)min(max(267 - (int)eb, 1), 253);
 }
 
-// The q parts of (entry b, columns from c0) and each column's scale, lse and limit,
+// The q parts of (entry b, columns from c0) and each column's scale, -lse and limit,
 // rows dealt to the compute warps.
 template <bool Q8, int NC>
 __device__ __forceinline__ void fill_q(const MassArgs& a, char* sm, uint32_t warp, uint32_t lane, uint32_t b, uint32_t c0,
@@ -275,8 +290,10 @@ __device__ __forceinline__ void fill_q(const MassArgs& a, char* sm, uint32_t war
     if (lane == 0) {
       const float l = live ? a.lse[(uint64_t)b * cols + c] : -INFINITY;
       const uint32_t behind = a.n_q - 1 - c / a.n_heads;  // positions behind the column's query
-      col[r] = a.scale * __uint_as_float((254u - f2) << 23);
-      col[M::RB + r] = l;
+      // exp(s - lse) = 2^(s log2 e - lse log2 e)
+      constexpr double LOG2E = 1.4426950408889634;
+      col[2 * r] = (float)(a.scale * LOG2E) * __uint_as_float((254u - f2) << 23);
+      col[2 * r + 1] = (float)(-l * LOG2E);
       // a column past the last, or a query that saw nothing, has no positions
       reinterpret_cast<uint32_t*>(col)[2 * M::RB + r] = l == -INFINITY || len <= behind ? 0u : len - behind;
     }
@@ -427,13 +444,17 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         __syncwarp();
         if (lane == 0) kvtc::mbar_arrive(bar(M::B_TE));
         if (d.p0 + pair * HALF >= d.end) continue;
-#pragma unroll 1
-        for (uint32_t s = 0; ok && s < STEPS; ++s, ++j) {
-          const uint32_t f = j & 1u;
+        // the warpgroups' blocks as they come
+        uint32_t done[2] = {0, 0};  // steps issued
+        long long t0 = 0;
+        while (done[0] + done[1] < 2 * STEPS) {
+          bool any = false;
 #pragma unroll
           for (uint32_t g = 0; g < 2; ++g) {
-            const uint32_t wg = 2 * pair + g;
-            if (!(ok = wait(M::B_AF + 2 * wg + f, (j >> 1) & 1u))) break;
+            const uint32_t wg = 2 * pair + g, s = done[g], f = (j + s) & 1u;
+            if (s == STEPS || !try_all(bar(M::B_AF + 2 * wg + f), ((j + s) >> 1) & 1u)) continue;
+            any = true;
+            ++done[g];
             kvtc::tc_fence_after();
             if (kvtc::elect_one()) {
               const uint32_t ta = tmem + wg * TM_WG + f * M::A_COLS, td = tmem + wg * TM_WG + M::TM_D + f * M::N;
@@ -450,7 +471,17 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             }
             __syncwarp();
           }
+          if (any) {
+            t0 = 0;
+          } else if (t0 == 0) {
+            t0 = clock64();
+          } else if (__any_sync(0xffffffffu, *abort_flag || clock64() - t0 > t.wait_limit)) {
+            *abort_flag = 1u;
+            ok = false;
+            break;
+          }
         }
+        j += STEPS;
       }
       // all issued MMAs retire before TMEM is freed
       if (kvtc::elect_one()) kvtc::mma_commit(bar(M::B_FINAL + pair));
@@ -468,7 +499,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     float* give = reinterpret_cast<float*>(sm + M::X) + wg * HC * HALF + r;
     const float* got = reinterpret_cast<const float*>(sm + M::X) + (wg ^ 1u) * HC * HALF + r;
     float* sums = reinterpret_cast<float*>(sm + M::S) + pair * 2 * HALF + r;
-    const float* col = reinterpret_cast<const float*>(sm + M::COL) + g * HC;
+    const float2* col = reinterpret_cast<const float2*>(sm + M::COL) + g * HC;  // scale, -lse in powers of two
+    const uint32_t* limit = reinterpret_cast<const uint32_t*>(sm + M::COL) + 2 * M::RB + g * HC;
     uint32_t j = 0, ui = 0, xi = 0;  // steps of the warpgroup, units of its ring, finished tiles of the pair
     // the first warpgroup: the tile before, whose mass is written once the other's sum is there
     float* out = nullptr;
@@ -518,10 +550,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       __syncwarp();
       if (lane == 0) kvtc::mbar_arrive(bar(M::B_XE + pair));
       float sum = 0.f;
+      // a column that is not there has -lse = +inf and limit 0; with one query all others' limit is the length
 #pragma unroll
-      for (int c = 0; c < HC; ++c)
-        if (d_p < reinterpret_cast<const uint32_t*>(col)[2 * M::RB + c])
-          sum += expf(fmaf(mine[c], col[c], -col[M::RB + c]));
+      for (int c = 0; c < HC; ++c) {
+        const float2 k = col[c];
+        const float w = exp2_approx(fmaf(mine[c], k.x, k.y));
+        sum += (a.n_q == 1 ? k.y != INFINITY : d_p < limit[c]) ? w : 0.f;
+      }
       if (g) {
         sums[(xi & 1u) * HALF] = sum;
       } else {
