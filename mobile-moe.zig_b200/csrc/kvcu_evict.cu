@@ -38,7 +38,7 @@ __device__ __forceinline__ uint32_t ld_cluster(const uint32_t* p, uint32_t rank)
 struct SelectArgs {
   const float* mass;
   uint64_t mass_lstride, mass_stride;
-  uint32_t n, n_seqs;
+  uint32_t n_layers, n, n_seqs;
   const uint32_t* seq_ids;
   const uint32_t* lens;
   uint32_t budget, n_sink, n_recent;
@@ -46,48 +46,67 @@ struct SelectArgs {
   uint64_t keep_lstride, keep_stride;
   uint32_t* counts;
   uint32_t* status;
-  uint32_t cap;  // positions a CTA's shared memory holds
+  uint32_t cap;  // groups of four positions a CTA's shared memory holds
 };
 
 constexpr uint32_t BINS = 2048;
+constexpr uint32_t ORDERED = 512;  // entries up to which rows are taken longest first
+constexpr uint32_t SHARED_KEYS = 22528;  // 88 KB
+constexpr int SELECT_THREADS = 512;
 
 // Ascending 32-bit order of the values; -0 and +0 are one value, NaN is below
 // everything.
 __device__ __forceinline__ uint32_t order_key(float v) {
-  if (v != v) return 0u;
-  const uint32_t b = __float_as_uint(v + 0.0f);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+  const int b = __float_as_int(v + 0.0f);
+  return v == v ? (uint32_t)(b ^ ((b >> 31) | (int)0x80000000)) : 0u;
 }
 
-// Inclusive sum over the block of one value per thread.  `part` holds one word
-// per warp; ends with a barrier before `part` may be reused.
-template <int NT>
-__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* part) {
-  const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+__device__ __forceinline__ uint32_t warp_scan(uint32_t v, uint32_t lane) {
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const uint32_t y = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= (uint32_t)o) v += y;
   }
-  if (lane == 31) part[warp] = v;
-  __syncthreads();
-  uint32_t before = 0;
-  for (uint32_t w = 0; w < warp; ++w) before += part[w];
-  __syncthreads();
-  return v + before;
+  return v;
+}
+
+// Sum of the block's earlier warps' words part[w] (every warp scans them for itself).
+template <int NT>
+__device__ __forceinline__ uint32_t before_warp(const uint32_t* part, uint32_t warp, uint32_t lane) {
+  const uint32_t p = lane < NT / 32 ? part[lane] : 0u;
+  return __shfl_sync(0xffffffffu, warp_scan(p, lane) - p, warp);
 }
 
 // One row per cluster of C CTAs; each CTA holds an equal share of the row's
 // middle, in order.
 template <int C, int NT>
-__global__ void __launch_bounds__(NT) k_evict_select(SelectArgs a) {
-  extern __shared__ uint32_t cache[];  // [cap] order keys of this CTA's share
+__global__ void __launch_bounds__(NT, 2) k_evict_select(SelectArgs a) {
+  extern __shared__ uint4 cache[];  // [cap] order keys of this CTA's share, four positions each
   __shared__ uint32_t hist[BINS], total[BINS];
   __shared__ uint32_t part[NT / 32], part2[NT / 32];
   __shared__ uint32_t s_bin, s_above, s_tot[2];
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
   const uint32_t rank = C > 1 ? cluster_rank() : 0u;
-  const uint32_t row = blockIdx.x / C, layer = row / a.n, b = row % a.n;
+  const uint32_t row = blockIdx.x / C;
+  uint32_t layer = row / a.n, b = row % a.n;
+  if (a.n > 1 && a.n <= ORDERED) {
+    // long rows first, so that none starts when the others end: all layers of the
+    // entry whose length has rank row / layers (a few loads and compares per CTA)
+    for (uint32_t i = tid; i < a.n; i += NT) {
+      const uint32_t q = a.seq_ids ? a.seq_ids[i] : i;
+      total[i] = q < a.n_seqs ? a.lens[q] : 0u;
+    }
+    __syncthreads();
+    layer = row % a.n_layers;
+    for (uint32_t i = tid; i < a.n; i += NT) {
+      const uint32_t mine = total[i];
+      uint32_t rank_i = 0;
+      for (uint32_t k = 0; k < a.n; ++k) rank_i += total[k] > mine || (total[k] == mine && k < i);
+      if (rank_i == row / a.n_layers) s_bin = i;
+    }
+    __syncthreads();
+    b = s_bin;
+  }
   const uint32_t s = a.seq_ids ? a.seq_ids[b] : b;
   uint32_t len = 0;
   if (s < a.n_seqs) {
@@ -115,7 +134,39 @@ __global__ void __launch_bounds__(NT) k_evict_select(SelectArgs a) {
   const uint32_t share = (hi - lo + C - 1) / C;
   const uint32_t p0 = min(lo + rank * share, hi), p1 = min(p0 + share, hi), cnt = p1 - p0;
   const float* mass = a.mass + layer * a.mass_lstride + b * a.mass_stride + p0;
-  auto key_at = [&](uint32_t i) { return i < a.cap ? cache[i] : order_key(mass[i]); };
+  // The share in groups of four positions that are 16-byte aligned in memory: position
+  // v = 4 g + j - off of it, which the first and last group may only have in part.
+  const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(mass) >> 2) & 3u;
+  const uint32_t groups = (cnt + off + 3) / 4;
+  auto read = [&](uint32_t g) -> float4 {
+    const uint32_t v = 4 * g - off;
+    if (v < cnt && v + 4 <= cnt) return *reinterpret_cast<const float4*>(mass + v);
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (v < cnt) x.x = mass[v];
+    if (v + 1 < cnt) x.y = mass[v + 1];
+    if (v + 2 < cnt) x.z = mass[v + 2];
+    if (v + 3 < cnt) x.w = mass[v + 3];
+    return x;
+  };
+  auto keys_of = [&](float4 x) {
+    return make_uint4(order_key(x.x), order_key(x.y), order_key(x.z), order_key(x.w));
+  };
+  auto keys_at = [&](uint32_t g) -> uint4 { return g < a.cap ? cache[g] : keys_of(read(g)); };
+  // f(key) for the group's positions that are there
+  auto each = [&](uint32_t g, const uint4& k, auto&& f) {
+    const uint32_t v = 4 * g - off;
+    if (v + 4 <= cnt && v < cnt) {
+      f(k.x);
+      f(k.y);
+      f(k.z);
+      f(k.w);
+      return;
+    }
+    if (v < cnt) f(k.x);
+    if (v + 1 < cnt) f(k.y);
+    if (v + 2 < cnt) f(k.z);
+    if (v + 3 < cnt) f(k.w);
+  };
 
   // ---- radix select of the need-th largest key
   uint32_t prefix = 0, above = 0;  // keys above the prefix's range: all kept
@@ -125,17 +176,33 @@ __global__ void __launch_bounds__(NT) k_evict_select(SelectArgs a) {
     const uint32_t mask = pass == 2 ? 1023u : 2047u;
     for (uint32_t i = tid; i < BINS; i += NT) hist[i] = 0;
     __syncthreads();
-    if (pass == 0) {
-      for (uint32_t i = tid; i < cnt; i += NT) {
-        const uint32_t k = order_key(mass[i]);
-        if (i < a.cap) cache[i] = k;
-        atomicAdd(&hist[k >> 21], 1u);
-      }
-    } else {
-      const int top = pass == 1 ? 21 : 10;
-      for (uint32_t i = tid; i < cnt; i += NT) {
-        const uint32_t k = key_at(i);
-        if ((k >> top) == prefix) atomicAdd(&hist[(k >> shift) & mask], 1u);
+    constexpr uint32_t U = 4;  // groups of a thread in flight
+    for (uint32_t g0 = tid; g0 < groups; g0 += U * NT) {
+      uint4 k[U];
+      if (pass == 0) {
+        float4 x[U];
+#pragma unroll
+        for (uint32_t j = 0; j < U; ++j)
+          if (g0 + j * NT < groups) x[j] = read(g0 + j * NT);
+#pragma unroll
+        for (uint32_t j = 0; j < U; ++j) {
+          const uint32_t g = g0 + j * NT;
+          if (g >= groups) break;
+          const uint4 key = keys_of(x[j]);
+          if (g < a.cap) cache[g] = key;
+          each(g, key, [&](uint32_t v) { atomicAdd(&hist[v >> 21], 1u); });
+        }
+      } else {
+        const int top = pass == 1 ? 21 : 10;
+#pragma unroll
+        for (uint32_t j = 0; j < U; ++j)
+          if (g0 + j * NT < groups) k[j] = keys_at(g0 + j * NT);
+#pragma unroll
+        for (uint32_t j = 0; j < U; ++j)
+          if (g0 + j * NT < groups)
+            each(g0 + j * NT, k[j], [&](uint32_t v) {
+              if ((v >> top) == prefix) atomicAdd(&hist[(v >> shift) & mask], 1u);
+            });
       }
     }
     const uint32_t* h = hist;
@@ -161,9 +228,11 @@ __global__ void __launch_bounds__(NT) k_evict_select(SelectArgs a) {
       own[j] = bin <= mask ? h[bin] : 0u;
       mine += own[j];
     }
-    const uint32_t upto = block_scan<NT>(mine, part);
-    uint32_t run = above + upto - mine;
-    if (run < need && need <= above + upto) {
+    const uint32_t in_warp = warp_scan(mine, lane);
+    if (lane == 31) part[warp] = in_warp;
+    __syncthreads();
+    uint32_t run = above + before_warp<NT>(part, warp, lane) + in_warp - mine;
+    if (run < need && need <= run + mine) {
 #pragma unroll
       for (uint32_t j = 0; j < PER; ++j) {
         if (run < need && need <= run + own[j]) {
@@ -176,18 +245,24 @@ __global__ void __launch_bounds__(NT) k_evict_select(SelectArgs a) {
     __syncthreads();
     prefix = (prefix << (pass == 2 ? 10 : 11)) | s_bin;
     above = s_above;
-    __syncthreads();
   }
   const uint32_t ties = need - above;  // of the positions equal to the threshold, the first `ties`
 
-  // ---- the kept positions in order: each warp takes a run of the share
-  const uint32_t run = ((cnt + NT / 32 - 1) / (NT / 32) + 31u) & ~31u;
-  const uint32_t w0 = min(warp * run, cnt), w1 = min(w0 + run, cnt);
+  // ---- the kept positions in order: each warp takes a run of the groups.  Counts go
+  // in pairs, those above the threshold in the low half of a word, equal ones in the high.
+  const uint32_t run = (groups + NT - 1) / NT * 32u;
+  const uint32_t w0 = min(warp * run, groups), w1 = min(w0 + run, groups);
+  auto pair_of = [&](uint32_t g, const uint4& k) {
+    uint32_t n = 0;
+    each(g, k, [&](uint32_t v) { n += v > prefix ? 1u : v == prefix ? 0x10000u : 0u; });
+    return n;
+  };
   uint32_t gt = 0, eq = 0;
-  for (uint32_t i = w0 + lane; i < w1; i += 32) {
-    const uint32_t k = key_at(i);
-    gt += k > prefix;
-    eq += k == prefix;
+#pragma unroll 4
+  for (uint32_t g = w0 + lane; g < w1; g += 32) {
+    const uint32_t n = pair_of(g, keys_at(g));
+    gt += n & 0xFFFFu;
+    eq += n >> 16;
   }
   gt = __reduce_add_sync(0xffffffffu, gt);
   eq = __reduce_add_sync(0xffffffffu, eq);
@@ -196,11 +271,7 @@ __global__ void __launch_bounds__(NT) k_evict_select(SelectArgs a) {
     part2[warp] = eq;
   }
   __syncthreads();
-  uint32_t gt0 = 0, eq0 = 0;
-  for (uint32_t w = 0; w < warp; ++w) {
-    gt0 += part[w];
-    eq0 += part2[w];
-  }
+  uint32_t gt0 = before_warp<NT>(part, warp, lane), eq0 = before_warp<NT>(part2, warp, lane);
   if constexpr (C > 1) {
     if (tid == NT - 1) {
       s_tot[0] = gt0 + gt;
@@ -213,16 +284,29 @@ __global__ void __launch_bounds__(NT) k_evict_select(SelectArgs a) {
     }
     cluster_sync();  // no CTA leaves while another reads its shared memory
   }
-  const uint32_t below = (1u << lane) - 1u;
-  for (uint32_t i0 = w0; i0 < w1; i0 += 32) {
-    const uint32_t i = i0 + lane;
-    const uint32_t k = i < w1 ? key_at(i) : 0u;
-    const bool g = i < w1 && k > prefix, e = i < w1 && k == prefix;
-    const uint32_t mg = __ballot_sync(0xffffffffu, g), me = __ballot_sync(0xffffffffu, e);
-    const uint32_t gi = gt0 + __popc(mg & below), ei = eq0 + __popc(me & below);
-    if (g || (e && ei < ties)) keep[a.n_sink + gi + min(ei, ties)] = p0 + i;
-    gt0 += __popc(mg);
-    eq0 += __popc(me);
+  for (uint32_t g0 = w0; g0 < w1; g0 += 32) {
+    const uint32_t g = g0 + lane;
+    const uint4 k = g < w1 ? keys_at(g) : make_uint4(0, 0, 0, 0);
+    const uint32_t n = g < w1 ? pair_of(g, k) : 0u;
+    const uint32_t upto = warp_scan(n, lane), all = __shfl_sync(0xffffffffu, upto, 31);
+    uint32_t gi = gt0 + ((upto - n) & 0xFFFFu), ei = eq0 + ((upto - n) >> 16);
+    if (n) {
+      uint32_t p = p0 + 4 * g - off;  // of the group's first position
+      const uint32_t kk[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j, ++p) {
+        if (p - p0 >= cnt) continue;
+        if (kk[j] > prefix) {
+          keep[a.n_sink + gi + min(ei, ties)] = p;
+          ++gi;
+        } else if (kk[j] == prefix) {
+          if (ei < ties) keep[a.n_sink + gi + ei] = p;
+          ++ei;
+        }
+      }
+    }
+    gt0 += all & 0xFFFFu;
+    eq0 += all >> 16;
   }
 }
 
@@ -304,49 +388,59 @@ __global__ void __launch_bounds__(CT) k_evict_compact(CompactArgs a, uint32_t C)
   const uint32_t stage = a.tile * (a.row_a + pad_b);
   const uint32_t waves = (count + C * a.tile - 1) / (C * a.tile);
 
-  auto row_of = [&](uint32_t p) -> uint64_t {
-    const uint32_t bi = p / a.block_size;
-    if (bi >= t1 - t0) {
+  // Thread r < tile has row r of the CTA's tile.  Its numbers run ahead of the
+  // copies: the list is read three waves, the block table two waves before they are
+  // needed, and neither is waited for until then.
+  auto row_j = [&](uint32_t w) { return (w * C + rank) * a.tile + tid; };
+  uint32_t pos, at = KVCU_NO_POSITION, blk_src = 0, blk_dst = 0;  // position fetched; position resolved, its blocks
+  float val = 0.0f;
+  auto fetch = [&](uint32_t w) { pos = tid < a.tile && row_j(w) < count ? keep[row_j(w)] : KVCU_NO_POSITION; };
+  auto resolve = [&](uint32_t w) {
+    const uint32_t j = row_j(w);
+    at = pos == j ? KVCU_NO_POSITION : pos;  // a row that is in its place stays there
+    if (at == KVCU_NO_POSITION) return;
+    if (at / a.block_size >= t1 - t0 || j / a.block_size >= t1 - t0) {
       atomicOr(a.status, KVCU_STATUS_BAD_TABLE);
-      return NO_ROW;
+      at = KVCU_NO_POSITION;
+      return;
     }
-    const uint32_t blk = a.tables[t0 + bi];
-    if (blk >= a.num_blocks) {
-      atomicOr(a.status, KVCU_STATUS_BAD_BLOCK);
-      return NO_ROW;
-    }
-    return base + (uint64_t)blk * a.block_size + p % a.block_size;
+    blk_src = a.tables[t0 + at / a.block_size];
+    blk_dst = a.tables[t0 + j / a.block_size];
+    if (mass) val = at < a.mass_stride ? __ldcg(mass + at) : 0.0f;
   };
-  auto load = [&](uint32_t w) {
+  auto load = [&](uint32_t w) {  // the copies of wave w, resolved before
     const uint32_t f = w & 1u;
-    const uint32_t j0 = (w * C + rank) * a.tile;
     if (tid < a.tile) {
       uint64_t src = NO_ROW, dst = NO_ROW;
-      const uint32_t j = j0 + tid;
-      if (j < count) {
-        const uint32_t p = keep[j];
-        if (p != j) {
-          src = row_of(p);
-          dst = row_of(j);
-          if (src == NO_ROW) dst = NO_ROW;
-          if (mass) mval[f][tid] = p < a.mass_stride ? __ldcg(mass + p) : 0.0f;
+      if (at != KVCU_NO_POSITION) {
+        if (blk_src < a.num_blocks && blk_dst < a.num_blocks) {
+          src = base + (uint64_t)blk_src * a.block_size + at % a.block_size;
+          dst = base + (uint64_t)blk_dst * a.block_size + row_j(w) % a.block_size;
+        } else {
+          atomicOr(a.status, KVCU_STATUS_BAD_BLOCK);
         }
       }
       src_row[f][tid] = src;
       dst_row[f][tid] = dst;
+      mval[f][tid] = val;
     }
     __syncthreads();
+    if (w + 1 < waves) resolve(w + 1);
+    if (w + 2 < waves) fetch(w + 2);
     char* st = smem + f * stage;
     const uint32_t sa = static_cast<uint32_t>(__cvta_generic_to_shared(st));
     for (uint32_t r = warp; r < a.tile; r += CT / 32) {
       const uint64_t src = src_row[f][r];
-      if (dst_row[f][r] == NO_ROW) continue;
+      if (src == NO_ROW) continue;
       for (uint32_t o = lane * UA; o < a.row_a; o += 32 * UA) copy_in<UA>(sa + r * a.row_a + o, a.a + src * a.row_a + o);
       const uint32_t sb = sa + a.tile * a.row_a + r * pad_b;
       for (uint32_t o = lane * UB; o < a.row_b; o += 32 * UB) copy_in<UB>(sb + o, a.b + src * a.row_b + o);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  fetch(0);
+  resolve(0);
+  if (waves > 1) fetch(1);
   load(0);
   for (uint32_t w = 0; w < waves; ++w) {
     if (w + 1 < waves) {
@@ -372,6 +466,170 @@ __global__ void __launch_bounds__(CT) k_evict_compact(CompactArgs a, uint32_t C)
       if (j < a.mass_stride) mass[j] = mval[f][tid];
     }
     __syncthreads();  // the stage may be filled again
+  }
+}
+
+// ---- the same through registers: a thread has the same pieces of a tile's rows in
+// every wave (up to four of 32 bytes and two of 4), so a wave costs it a handful of
+// 256-bit loads and stores and no pass through shared memory; the next wave's loads
+// are in flight while one is written.
+struct Piece {
+  char* base;        // of the array, at the piece's place in a row
+  uint32_t pitch;    // bytes of a row
+  uint32_t row;      // of the tile; NO_PIECE: none
+};
+constexpr uint32_t NO_PIECE = 0xFFFFFFFFu;
+constexpr int WIDE = 4, WORDS = 2;
+constexpr uint32_t REG_TILE = 56;  // rows at most
+
+struct Wave {
+  uint32_t wide[WIDE][8];
+  uint32_t word[WORDS];
+};
+
+__device__ __forceinline__ void ld256(uint32_t (&v)[8], const char* p) {
+  asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "l"(p)
+               : "memory");
+}
+__device__ __forceinline__ void st256(char* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+__global__ void __launch_bounds__(CT, 2) k_evict_compact_wide(CompactArgs a, uint32_t C) {
+  __shared__ uint64_t src_row[2][REG_TILE], dst_row[2][REG_TILE];
+  const uint32_t tid = threadIdx.x;
+  const uint32_t rank = C > 1 ? cluster_rank() : 0u;
+  const uint32_t pair = blockIdx.x / C, layer = pair / a.n, b = pair % a.n;
+  const uint32_t s = a.seq_ids ? a.seq_ids[b] : b;
+  if (s >= a.n_seqs) {
+    if (tid == 0) atomicOr(a.status, KVCU_STATUS_BAD_SEQ);
+    return;
+  }
+  uint32_t count = a.counts[b];
+  if (count > a.keep_stride) {
+    if (tid == 0) atomicOr(a.status, KVCU_STATUS_BAD_LEN);
+    count = (uint32_t)a.keep_stride;
+  }
+  if (a.lens && layer == 0 && rank == 0 && tid == 0) a.lens[s] = count;
+  const uint32_t* keep = a.keep + layer * a.keep_lstride + b * a.keep_stride;
+  if (count == 0 || keep[count - 1] == count - 1) return;  // ascending: every row is in its place
+  const uint32_t t0 = a.toff[s], t1 = max(a.toff[s + 1], t0);
+  float* mass = a.mass ? a.mass + layer * a.mass_lstride + b * a.mass_stride : nullptr;
+  const uint64_t base = (uint64_t)(a.layer + layer) * a.layer_rows;
+  const uint32_t waves = (count + C * a.tile - 1) / (C * a.tile);
+  // this thread's pieces: 32-byte ones of the first array, then of the second where its rows have
+  // such; 4-byte words of the second otherwise
+  const uint32_t ca = a.row_a / 32, cb = a.row_b % 32 ? 0u : a.row_b / 32, wb = cb ? 0u : a.row_b / 4;
+  Piece wide[WIDE], word[WORDS];
+#pragma unroll
+  for (int i = 0; i < WIDE; ++i) {
+    const uint32_t k = tid + i * CT, na = a.tile * ca;
+    if (k < na) wide[i] = {a.a + k % ca * 32, a.row_a, k / ca};
+    else if (k - na < a.tile * cb) wide[i] = {a.b + (k - na) % cb * 32, a.row_b, (k - na) / cb};
+    else wide[i] = {nullptr, 0, NO_PIECE};
+  }
+#pragma unroll
+  for (int i = 0; i < WORDS; ++i) {
+    const uint32_t k = tid + i * CT;
+    if (k < a.tile * wb) word[i] = {a.b + k % wb * 4, a.row_b, k / wb};
+    else word[i] = {nullptr, 0, NO_PIECE};
+  }
+  // Thread r < tile has row r of the CTA's tile.  Its numbers run ahead of the
+  // copies: the list is read three waves, the block table two waves before they are
+  // needed, and neither is waited for until then.
+  auto row_j = [&](uint32_t w) { return (w * C + rank) * a.tile + tid; };
+  uint32_t pos = KVCU_NO_POSITION, at = KVCU_NO_POSITION, blk_src = 0, blk_dst = 0;
+  float val[2] = {0.0f, 0.0f}, val_next = 0.0f;
+  auto fetch = [&](uint32_t w) {
+    pos = w < waves && tid < a.tile && row_j(w) < count ? keep[row_j(w)] : KVCU_NO_POSITION;
+  };
+  auto resolve = [&](uint32_t w) {
+    const uint32_t j = row_j(w);
+    at = pos == j ? KVCU_NO_POSITION : pos;  // a row that is in its place stays there
+    if (at == KVCU_NO_POSITION) return;
+    if (at / a.block_size >= t1 - t0 || j / a.block_size >= t1 - t0) {
+      atomicOr(a.status, KVCU_STATUS_BAD_TABLE);
+      at = KVCU_NO_POSITION;
+      return;
+    }
+    blk_src = a.tables[t0 + at / a.block_size];
+    blk_dst = a.tables[t0 + j / a.block_size];
+    if (mass) val_next = at < a.mass_stride ? __ldcg(mass + at) : 0.0f;
+  };
+  auto publish = [&](uint32_t w, float& v) {
+    if (tid >= a.tile) return;
+    uint64_t src = NO_ROW, dst = NO_ROW;
+    if (at != KVCU_NO_POSITION) {
+      if (blk_src < a.num_blocks && blk_dst < a.num_blocks) {
+        src = base + (uint64_t)blk_src * a.block_size + at % a.block_size;
+        dst = base + (uint64_t)blk_dst * a.block_size + row_j(w) % a.block_size;
+      } else {
+        atomicOr(a.status, KVCU_STATUS_BAD_BLOCK);
+      }
+    }
+    src_row[w & 1u][tid] = src;
+    dst_row[w & 1u][tid] = dst;
+    v = val_next;
+  };
+  auto load = [&](uint32_t w, Wave& v) {
+#pragma unroll
+    for (int i = 0; i < WIDE; ++i) {
+      if (wide[i].row == NO_PIECE) continue;
+      const uint64_t r = src_row[w & 1u][wide[i].row];
+      if (r != NO_ROW) ld256(v.wide[i], wide[i].base + r * wide[i].pitch);
+    }
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) {
+      if (word[i].row == NO_PIECE) continue;
+      const uint64_t r = src_row[w & 1u][word[i].row];
+      if (r != NO_ROW) v.word[i] = *reinterpret_cast<const volatile uint32_t*>(word[i].base + r * word[i].pitch);
+    }
+  };
+  auto store = [&](uint32_t w, const Wave& v, float m) {
+#pragma unroll
+    for (int i = 0; i < WIDE; ++i) {
+      if (wide[i].row == NO_PIECE) continue;
+      const uint64_t r = dst_row[w & 1u][wide[i].row];
+      if (r != NO_ROW) st256(wide[i].base + r * wide[i].pitch, v.wide[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) {
+      if (word[i].row == NO_PIECE) continue;
+      const uint64_t r = dst_row[w & 1u][word[i].row];
+      if (r != NO_ROW) *reinterpret_cast<volatile uint32_t*>(word[i].base + r * word[i].pitch) = v.word[i];
+    }
+    if (mass && tid < a.tile && dst_row[w & 1u][tid] != NO_ROW && row_j(w) < a.mass_stride) mass[row_j(w)] = m;
+  };
+  Wave even, odd;
+  fetch(0);
+  resolve(0);
+  fetch(1);
+  publish(0, val[0]);
+  __syncthreads();
+  load(0, even);
+  resolve(1);
+  fetch(2);
+  // one wave: the next one's loads are sent, the cluster meets with this one's in registers, it is written
+  auto step = [&](uint32_t w, Wave& now, Wave& next, float& v, float& v_next) {
+    if (w + 1 < waves) {
+      publish(w + 1, v_next);
+      __syncthreads();
+      load(w + 1, next);
+      resolve(w + 2);
+      fetch(w + 3);
+    }
+    if (C > 1) cluster_sync();
+    else __syncthreads();
+    store(w, now, v);
+    __syncthreads();  // this wave's row numbers may be replaced
+  };
+  for (uint32_t w = 0; w < waves; w += 2) {
+    step(w, even, odd, val[0], val[1]);
+    if (w + 1 < waves) step(w + 1, odd, even, val[1], val[0]);
   }
 }
 
@@ -414,7 +672,7 @@ int launch_clusters(void (*kernel)(KArgs...), uint32_t clusters, uint32_t C, int
 
 template <int C>
 int launch_select(const SelectArgs& a, uint32_t rows, cudaStream_t st) {
-  return launch_clusters(k_evict_select<C, 1024>, rows, C, 1024, (size_t)a.cap * 4, st, "evict select launch", a);
+  return launch_clusters(k_evict_select<C, SELECT_THREADS>, rows, C, SELECT_THREADS, (size_t)a.cap * 16, st, "evict select launch", a);
 }
 
 template <int UA>
@@ -448,15 +706,17 @@ extern "C" int kvcu_evict_select(kvcu_pool* pool, uint32_t n_layers, uint32_t n,
   }
   DevScope d(pool->device);
   if (d.rc) return d.rc;
-  // CTAs of a row: a long row is shared until its keys fit the shared memory or
-  // the shares get short; few rows are shared to occupy more SMs.
+  // CTAs of a row: few rows are shared to occupy the SMs, while the shares are not too short
   const uint64_t sms = (uint64_t)kvcu_current_sm_count();
   uint32_t C = 1;
-  while (C < 8 && (mass_stride / C > KVCU_EVICT_SMEM / 4 || (rows * C * 2 <= sms && mass_stride / C > 4096))) C *= 2;
-  SelectArgs a = {mass, mass_layer_stride, mass_stride, n, n_seqs, seq_ids, lens, budget, n_sink, n_recent, keep,
+  while (C < 8 && rows * C <= sms && mass_stride / C > 4096) C *= 2;
+  SelectArgs a = {mass, mass_layer_stride, mass_stride, n_layers, n, n_seqs, seq_ids, lens, budget, n_sink, n_recent, keep,
                   keep_layer_stride, keep_stride, keep_counts, pool->status, 0};
   const uint64_t share = (mass_stride + C - 1) / C;
-  a.cap = share < KVCU_EVICT_SMEM / 4 ? (uint32_t)share : (uint32_t)(KVCU_EVICT_SMEM / 4);
+  // keys held in shared memory: with more CTAs than SMs two share an SM's, longer
+  // shares are read again from L2 in each pass
+  const uint64_t most = rows * C > sms ? SHARED_KEYS / 4 : KVCU_EVICT_SMEM / 16, need = share / 4 + 2;
+  a.cap = (uint32_t)(need < most ? need : most);
   const cudaStream_t st = (cudaStream_t)stream;
   if (C == 1) return launch_select<1>(a, (uint32_t)rows, st);
   if (C == 2) return launch_select<2>(a, (uint32_t)rows, st);
@@ -518,6 +778,22 @@ extern "C" int kvcu_evict_compact(kvcu_pool* pool, uint32_t layer, uint32_t n_la
   a.mass_stride = mass_stride;
   a.lens = lens;
   a.status = pool->status;
+  const uint64_t sms = (uint64_t)kvcu_current_sm_count();
+  const cudaStream_t st = (cudaStream_t)stream;
+  // Rows of whole 32-byte pieces, with a second array of such or of whole words (every
+  // Q8_0 pool of an even number of blocks, f32 pools of ranks divisible by 8), go through registers;
+  // 512 pairs of 2,048 kept rows of 612 B: COMPACT_WIDE us against 371 us through shared memory.
+  const uint32_t pieces = a.row_a / 32 + (a.row_b % 32 ? 0u : a.row_b / 32);
+  if (a.row_a % 32 == 0 && a.row_b % 4 == 0 && pieces <= WIDE * CT) {
+    a.tile = WIDE * CT / pieces;
+    if (a.row_b % 32 && a.tile > WORDS * CT / (a.row_b / 4)) a.tile = WORDS * CT / (a.row_b / 4);
+    if (a.tile > REG_TILE) a.tile = REG_TILE;
+    if (a.tile > 0) {
+      uint32_t C = 1;
+      while (C < 8 && pairs * C * 2 <= 4 * sms && (uint64_t)C * a.tile < keep_stride) C *= 2;
+      return launch_clusters(k_evict_compact_wide, (uint32_t)pairs, C, CT, 0, st, "evict compact launch", a, C);
+    }
+  }
   // two stages of about 20 KB, so that several CTAs share an SM
   const uint32_t row = a.row_a + ((a.row_b + 15u) & ~15u);
   uint32_t tile = 20480u / row;
@@ -529,10 +805,8 @@ extern "C" int kvcu_evict_compact(kvcu_pool* pool, uint32_t layer, uint32_t n_la
   }
   a.tile = tile;
   // CTAs of a pair: more while the grid stays within four CTAs an SM
-  const uint64_t sms = (uint64_t)kvcu_current_sm_count();
   uint32_t C = 1;
   while (C < 8 && pairs * C * 2 <= 4 * sms && (uint64_t)C * tile < keep_stride) C *= 2;
-  const cudaStream_t st = (cudaStream_t)stream;
   if (a.row_a % 16 == 0) return launch_compact<16>(a, (uint32_t)pairs, C, smem, st);
   return launch_compact<4>(a, (uint32_t)pairs, C, smem, st);
 }

@@ -178,6 +178,9 @@ def _keep_lists(rng, layers, lens, budget, kind):
     (False, (6, 10), 32, 1, [300], 100),
     (True, (33, 64), 32, 1, [300, 200], 64),
     (True, (96, 32), 48, 3, [333, 47], 48),
+    (True, (32, 64), 16, 2, [300, 77], 60),
+    (False, (128, 24), 16, 2, [300, 77], 60),
+    (False, (12, 8), 16, 1, [300], 160),
 ])
 def test_compact(kv, kind, quant, dims, bs, layers, lens, budget):
     import torch
