@@ -50,8 +50,9 @@ struct SelectArgs {
 };
 
 constexpr uint32_t BINS = 2048;
+constexpr uint32_t LIST = 2048;
 constexpr uint32_t ORDERED = 512;  // entries up to which rows are taken longest first
-constexpr uint32_t SHARED_KEYS = 22528;  // 88 KB
+constexpr uint32_t SHARED_KEYS = 18432;  // 72 KB
 constexpr int SELECT_THREADS = 512;
 
 // Ascending 32-bit order of the values; -0 and +0 are one value, NaN is below
@@ -84,7 +85,8 @@ __global__ void __launch_bounds__(NT, 2) k_evict_select(SelectArgs a) {
   extern __shared__ uint4 cache[];  // [cap] order keys of this CTA's share, four positions each
   __shared__ uint32_t hist[BINS], total[BINS];
   __shared__ uint32_t part[NT / 32], part2[NT / 32];
-  __shared__ uint32_t s_bin, s_above, s_tot[2];
+  __shared__ uint2 list[LIST];  // (key, position in the share) of the threshold's first bin
+  __shared__ uint32_t s_bin, s_above, s_listed, s_tot[2];
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
   const uint32_t rank = C > 1 ? cluster_rank() : 0u;
   const uint32_t row = blockIdx.x / C;
@@ -152,57 +154,87 @@ __global__ void __launch_bounds__(NT, 2) k_evict_select(SelectArgs a) {
     return make_uint4(order_key(x.x), order_key(x.y), order_key(x.z), order_key(x.w));
   };
   auto keys_at = [&](uint32_t g) -> uint4 { return g < a.cap ? cache[g] : keys_of(read(g)); };
-  // f(key) for the group's positions that are there
+  // f(key, position in the share) for the group's positions that are there
   auto each = [&](uint32_t g, const uint4& k, auto&& f) {
     const uint32_t v = 4 * g - off;
     if (v + 4 <= cnt && v < cnt) {
-      f(k.x);
-      f(k.y);
-      f(k.z);
-      f(k.w);
+      f(k.x, v);
+      f(k.y, v + 1);
+      f(k.z, v + 2);
+      f(k.w, v + 3);
       return;
     }
-    if (v < cnt) f(k.x);
-    if (v + 1 < cnt) f(k.y);
-    if (v + 2 < cnt) f(k.z);
-    if (v + 3 < cnt) f(k.w);
+    if (v < cnt) f(k.x, v);
+    if (v + 1 < cnt) f(k.y, v + 1);
+    if (v + 2 < cnt) f(k.z, v + 2);
+    if (v + 3 < cnt) f(k.w, v + 3);
   };
 
   // ---- radix select of the need-th largest key
+  // Warps take runs of the groups in order.  The first pass over the share forms the
+  // histogram of the keys' top 11 bits.  The second, knowing the threshold's bin,
+  // counts each run's keys above it and lists those in it, so that the finer
+  // histograms and the rest of the counts need only the list (where it overflows,
+  // they go over the whole share).  The last pass writes.
+  const uint32_t run = (groups + NT - 1) / NT * 32u;
+  const uint32_t w0 = min(warp * run, groups), w1 = min(w0 + run, groups);
+  if (tid == 0) s_listed = 0;
+  if (tid < NT / 32) part2[tid] = 0;
+  for (uint32_t i = tid; i < BINS; i += NT) hist[i] = 0;
+  __syncthreads();
+  constexpr uint32_t U = 4;  // groups of a thread in flight
+  for (uint32_t g0 = w0 + lane; g0 < w1; g0 += U * 32) {
+    float4 x[U];
+#pragma unroll
+    for (uint32_t j = 0; j < U; ++j)
+      if (g0 + j * 32 < w1) x[j] = read(g0 + j * 32);
+#pragma unroll
+    for (uint32_t j = 0; j < U; ++j) {
+      const uint32_t g = g0 + j * 32;
+      if (g >= w1) break;
+      const uint4 key = keys_of(x[j]);
+      if (g < a.cap) cache[g] = key;
+      each(g, key, [&](uint32_t v, uint32_t) { atomicAdd(&hist[v >> 21], 1u); });
+    }
+  }
   uint32_t prefix = 0, above = 0;  // keys above the prefix's range: all kept
+  uint32_t sure = 0;               // this lane's keys above the first bin
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, top = pass == 1 ? 21 : 10;
     const uint32_t mask = pass == 2 ? 1023u : 2047u;
-    for (uint32_t i = tid; i < BINS; i += NT) hist[i] = 0;
-    __syncthreads();
-    constexpr uint32_t U = 4;  // groups of a thread in flight
-    for (uint32_t g0 = tid; g0 < groups; g0 += U * NT) {
-      uint4 k[U];
-      if (pass == 0) {
-        float4 x[U];
+    if (pass) {
+      for (uint32_t i = tid; i < BINS; i += NT) hist[i] = 0;
+      if (pass == 1) {
+        const uint32_t lo = prefix << 21;
+        for (uint32_t g0 = w0 + lane; g0 < w1; g0 += U * 32) {
+          uint4 k[U];
 #pragma unroll
-        for (uint32_t j = 0; j < U; ++j)
-          if (g0 + j * NT < groups) x[j] = read(g0 + j * NT);
+          for (uint32_t j = 0; j < U; ++j)
+            if (g0 + j * 32 < w1) k[j] = keys_at(g0 + j * 32);
 #pragma unroll
-        for (uint32_t j = 0; j < U; ++j) {
-          const uint32_t g = g0 + j * NT;
-          if (g >= groups) break;
-          const uint4 key = keys_of(x[j]);
-          if (g < a.cap) cache[g] = key;
-          each(g, key, [&](uint32_t v) { atomicAdd(&hist[v >> 21], 1u); });
+          for (uint32_t j = 0; j < U; ++j)
+            if (g0 + j * 32 < w1)
+              each(g0 + j * 32, k[j], [&](uint32_t v, uint32_t at) {
+                if (v < lo) return;
+                if (v - lo >= 1u << 21) {
+                  ++sure;
+                } else {
+                  const uint32_t n = atomicAdd(&s_listed, 1u);
+                  if (n < LIST) list[n] = make_uint2(v, at);
+                }
+              });
         }
+      }
+      __syncthreads();
+      auto add = [&](uint32_t v) {
+        if ((v >> top) == prefix) atomicAdd(&hist[(v >> shift) & mask], 1u);
+      };
+      if (s_listed <= LIST) {
+        for (uint32_t i = tid; i < s_listed; i += NT) add(list[i].x);
       } else {
-        const int top = pass == 1 ? 21 : 10;
-#pragma unroll
-        for (uint32_t j = 0; j < U; ++j)
-          if (g0 + j * NT < groups) k[j] = keys_at(g0 + j * NT);
-#pragma unroll
-        for (uint32_t j = 0; j < U; ++j)
-          if (g0 + j * NT < groups)
-            each(g0 + j * NT, k[j], [&](uint32_t v) {
-              if ((v >> top) == prefix) atomicAdd(&hist[(v >> shift) & mask], 1u);
-            });
+#pragma unroll 4
+        for (uint32_t g = w0 + lane; g < w1; g += 32) each(g, keys_at(g), [&](uint32_t v, uint32_t) { add(v); });
       }
     }
     const uint32_t* h = hist;
@@ -231,15 +263,15 @@ __global__ void __launch_bounds__(NT, 2) k_evict_select(SelectArgs a) {
     const uint32_t in_warp = warp_scan(mine, lane);
     if (lane == 31) part[warp] = in_warp;
     __syncthreads();
-    uint32_t run = above + before_warp<NT>(part, warp, lane) + in_warp - mine;
-    if (run < need && need <= run + mine) {
+    uint32_t upto = above + before_warp<NT>(part, warp, lane) + in_warp - mine;
+    if (upto < need && need <= upto + mine) {
 #pragma unroll
       for (uint32_t j = 0; j < PER; ++j) {
-        if (run < need && need <= run + own[j]) {
+        if (upto < need && need <= upto + own[j]) {
           s_bin = BINS - 1 - (tid * PER + j);
-          s_above = run;
+          s_above = upto;
         }
-        run += own[j];
+        upto += own[j];
       }
     }
     __syncthreads();
@@ -248,34 +280,34 @@ __global__ void __launch_bounds__(NT, 2) k_evict_select(SelectArgs a) {
   }
   const uint32_t ties = need - above;  // of the positions equal to the threshold, the first `ties`
 
-  // ---- the kept positions in order: each warp takes a run of the groups.  Counts go
-  // in pairs, those above the threshold in the low half of a word, equal ones in the high.
-  const uint32_t run = (groups + NT - 1) / NT * 32u;
-  const uint32_t w0 = min(warp * run, groups), w1 = min(w0 + run, groups);
-  auto pair_of = [&](uint32_t g, const uint4& k) {
-    uint32_t n = 0;
-    each(g, k, [&](uint32_t v) { n += v > prefix ? 1u : v == prefix ? 0x10000u : 0u; });
-    return n;
-  };
-  uint32_t gt = 0, eq = 0;
+  // ---- how many each run keeps: keys above the threshold, and equal ones
+  if (s_listed > LIST) {
+    uint32_t eq = 0;
+    sure = 0;
 #pragma unroll 4
-  for (uint32_t g = w0 + lane; g < w1; g += 32) {
-    const uint32_t n = pair_of(g, keys_at(g));
-    gt += n & 0xFFFFu;
-    eq += n >> 16;
+    for (uint32_t g = w0 + lane; g < w1; g += 32)
+      each(g, keys_at(g), [&](uint32_t v, uint32_t) {
+        sure += v > prefix;
+        eq += v == prefix;
+      });
+    eq = __reduce_add_sync(0xffffffffu, eq);
+    if (lane == 0) part2[warp] = eq;
   }
-  gt = __reduce_add_sync(0xffffffffu, gt);
-  eq = __reduce_add_sync(0xffffffffu, eq);
-  if (lane == 0) {
-    part[warp] = gt;
-    part2[warp] = eq;
-  }
+  sure = __reduce_add_sync(0xffffffffu, sure);
+  if (lane == 0) part[warp] = sure;
   __syncthreads();
+  if (s_listed <= LIST) {
+    for (uint32_t i = tid; i < s_listed; i += NT) {
+      const uint2 e = list[i];
+      if (e.x >= prefix) atomicAdd(e.x > prefix ? &part[(e.y + off) / 4 / run] : &part2[(e.y + off) / 4 / run], 1u);
+    }
+    __syncthreads();
+  }
   uint32_t gt0 = before_warp<NT>(part, warp, lane), eq0 = before_warp<NT>(part2, warp, lane);
   if constexpr (C > 1) {
     if (tid == NT - 1) {
-      s_tot[0] = gt0 + gt;
-      s_tot[1] = eq0 + eq;
+      s_tot[0] = gt0 + part[warp];
+      s_tot[1] = eq0 + part2[warp];
     }
     cluster_sync();
     for (uint32_t r = 0; r < rank; ++r) {
@@ -284,26 +316,31 @@ __global__ void __launch_bounds__(NT, 2) k_evict_select(SelectArgs a) {
     }
     cluster_sync();  // no CTA leaves while another reads its shared memory
   }
+
+  // ---- the kept positions in order.  Counts go in pairs, those above the threshold in
+  // the low half of a word, equal ones in the high.
+  uint32_t* out = keep + a.n_sink;
+#pragma unroll 2
   for (uint32_t g0 = w0; g0 < w1; g0 += 32) {
     const uint32_t g = g0 + lane;
-    const uint4 k = g < w1 ? keys_at(g) : make_uint4(0, 0, 0, 0);
-    const uint32_t n = g < w1 ? pair_of(g, k) : 0u;
+    uint4 k = make_uint4(0, 0, 0, 0);
+    uint32_t n = 0;
+    if (g < w1) {
+      k = keys_at(g);
+      each(g, k, [&](uint32_t v, uint32_t) { n += v < prefix ? 0u : v == prefix ? 0x10000u : 1u; });
+    }
     const uint32_t upto = warp_scan(n, lane), all = __shfl_sync(0xffffffffu, upto, 31);
-    uint32_t gi = gt0 + ((upto - n) & 0xFFFFu), ei = eq0 + ((upto - n) >> 16);
     if (n) {
-      uint32_t p = p0 + 4 * g - off;  // of the group's first position
-      const uint32_t kk[4] = {k.x, k.y, k.z, k.w};
-#pragma unroll
-      for (uint32_t j = 0; j < 4; ++j, ++p) {
-        if (p - p0 >= cnt) continue;
-        if (kk[j] > prefix) {
-          keep[a.n_sink + gi + min(ei, ties)] = p;
+      uint32_t gi = gt0 + ((upto - n) & 0xFFFFu), ei = eq0 + ((upto - n) >> 16);
+      each(g, k, [&](uint32_t v, uint32_t at) {
+        if (v > prefix) {
+          out[gi + min(ei, ties)] = p0 + at;
           ++gi;
-        } else if (kk[j] == prefix) {
-          if (ei < ties) keep[a.n_sink + gi + ei] = p;
+        } else if (v == prefix) {
+          if (ei < ties) out[gi + ei] = p0 + at;
           ++ei;
         }
-      }
+      });
     }
     gt0 += all & 0xFFFFu;
     eq0 += all >> 16;
@@ -470,16 +507,14 @@ __global__ void __launch_bounds__(CT) k_evict_compact(CompactArgs a, uint32_t C)
 }
 
 // ---- the same through registers: a thread has the same pieces of a tile's rows in
-// every wave (up to four of 32 bytes and two of 4), so a wave costs it a handful of
+// every wave (up to three of 32 bytes and two of 4), so a wave costs it a handful of
 // 256-bit loads and stores and no pass through shared memory; the next wave's loads
 // are in flight while one is written.
-struct Piece {
-  char* base;        // of the array, at the piece's place in a row
-  uint32_t pitch;    // bytes of a row
-  uint32_t row;      // of the tile; NO_PIECE: none
-};
-constexpr uint32_t NO_PIECE = 0xFFFFFFFFu;
-constexpr int WIDE = 4, WORDS = 2;
+//
+// A piece is one word: its byte in the row, its row of the tile from bit 16, and
+// whether it lies in the second array.
+constexpr uint32_t SECOND = 0x80000000u, NO_PIECE = 0xFFFFFFFFu;
+constexpr int WIDE = 3, WORDS = 2;  // three CTAs an SM; with four pieces and two CTAs 348 us where this takes 251
 constexpr uint32_t REG_TILE = 56;  // rows at most
 
 struct Wave {
@@ -499,7 +534,7 @@ __device__ __forceinline__ void st256(char* p, const uint32_t (&v)[8]) {
                : "memory");
 }
 
-__global__ void __launch_bounds__(CT, 2) k_evict_compact_wide(CompactArgs a, uint32_t C) {
+__global__ void __launch_bounds__(CT, 3) k_evict_compact_wide(CompactArgs a, uint32_t C) {
   __shared__ uint64_t src_row[2][REG_TILE], dst_row[2][REG_TILE];
   const uint32_t tid = threadIdx.x;
   const uint32_t rank = C > 1 ? cluster_rank() : 0u;
@@ -524,20 +559,26 @@ __global__ void __launch_bounds__(CT, 2) k_evict_compact_wide(CompactArgs a, uin
   // this thread's pieces: 32-byte ones of the first array, then of the second where its rows have
   // such; 4-byte words of the second otherwise
   const uint32_t ca = a.row_a / 32, cb = a.row_b % 32 ? 0u : a.row_b / 32, wb = cb ? 0u : a.row_b / 4;
-  Piece wide[WIDE], word[WORDS];
+  uint32_t wide[WIDE], word[WORDS];
 #pragma unroll
   for (int i = 0; i < WIDE; ++i) {
     const uint32_t k = tid + i * CT, na = a.tile * ca;
-    if (k < na) wide[i] = {a.a + k % ca * 32, a.row_a, k / ca};
-    else if (k - na < a.tile * cb) wide[i] = {a.b + (k - na) % cb * 32, a.row_b, (k - na) / cb};
-    else wide[i] = {nullptr, 0, NO_PIECE};
+    if (k < na) wide[i] = k / ca << 16 | k % ca * 32;
+    else if (k - na < a.tile * cb) wide[i] = SECOND | (k - na) / cb << 16 | (k - na) % cb * 32;
+    else wide[i] = NO_PIECE;
   }
 #pragma unroll
   for (int i = 0; i < WORDS; ++i) {
     const uint32_t k = tid + i * CT;
-    if (k < a.tile * wb) word[i] = {a.b + k % wb * 4, a.row_b, k / wb};
-    else word[i] = {nullptr, 0, NO_PIECE};
+    word[i] = k < a.tile * wb ? k / wb << 16 | k % wb * 4 : NO_PIECE;
   }
+  auto row_in = [](uint32_t piece) { return piece >> 16 & 0xFFu; };
+  auto wide_at = [&](uint32_t piece, uint64_t r) {
+    return (piece & SECOND ? a.b + r * a.row_b : a.a + r * a.row_a) + (piece & 0xFFFFu);
+  };
+  auto word_at = [&](uint32_t piece, uint64_t r) {
+    return reinterpret_cast<volatile uint32_t*>(a.b + r * a.row_b + (piece & 0xFFFFu));
+  };
   // Thread r < tile has row r of the CTA's tile.  Its numbers run ahead of the
   // copies: the list is read three waves, the block table two waves before they are
   // needed, and neither is waited for until then.
@@ -578,29 +619,29 @@ __global__ void __launch_bounds__(CT, 2) k_evict_compact_wide(CompactArgs a, uin
   auto load = [&](uint32_t w, Wave& v) {
 #pragma unroll
     for (int i = 0; i < WIDE; ++i) {
-      if (wide[i].row == NO_PIECE) continue;
-      const uint64_t r = src_row[w & 1u][wide[i].row];
-      if (r != NO_ROW) ld256(v.wide[i], wide[i].base + r * wide[i].pitch);
+      if (wide[i] == NO_PIECE) continue;
+      const uint64_t r = src_row[w & 1u][row_in(wide[i])];
+      if (r != NO_ROW) ld256(v.wide[i], wide_at(wide[i], r));
     }
 #pragma unroll
     for (int i = 0; i < WORDS; ++i) {
-      if (word[i].row == NO_PIECE) continue;
-      const uint64_t r = src_row[w & 1u][word[i].row];
-      if (r != NO_ROW) v.word[i] = *reinterpret_cast<const volatile uint32_t*>(word[i].base + r * word[i].pitch);
+      if (word[i] == NO_PIECE) continue;
+      const uint64_t r = src_row[w & 1u][row_in(word[i])];
+      if (r != NO_ROW) v.word[i] = *word_at(word[i], r);
     }
   };
   auto store = [&](uint32_t w, const Wave& v, float m) {
 #pragma unroll
     for (int i = 0; i < WIDE; ++i) {
-      if (wide[i].row == NO_PIECE) continue;
-      const uint64_t r = dst_row[w & 1u][wide[i].row];
-      if (r != NO_ROW) st256(wide[i].base + r * wide[i].pitch, v.wide[i]);
+      if (wide[i] == NO_PIECE) continue;
+      const uint64_t r = dst_row[w & 1u][row_in(wide[i])];
+      if (r != NO_ROW) st256(wide_at(wide[i], r), v.wide[i]);
     }
 #pragma unroll
     for (int i = 0; i < WORDS; ++i) {
-      if (word[i].row == NO_PIECE) continue;
-      const uint64_t r = dst_row[w & 1u][word[i].row];
-      if (r != NO_ROW) *reinterpret_cast<volatile uint32_t*>(word[i].base + r * word[i].pitch) = v.word[i];
+      if (word[i] == NO_PIECE) continue;
+      const uint64_t r = dst_row[w & 1u][row_in(word[i])];
+      if (r != NO_ROW) *word_at(word[i], r) = v.word[i];
     }
     if (mass && tid < a.tile && dst_row[w & 1u][tid] != NO_ROW && row_j(w) < a.mass_stride) mass[row_j(w)] = m;
   };
@@ -782,9 +823,9 @@ extern "C" int kvcu_evict_compact(kvcu_pool* pool, uint32_t layer, uint32_t n_la
   const cudaStream_t st = (cudaStream_t)stream;
   // Rows of whole 32-byte pieces, with a second array of such or of whole words (every
   // Q8_0 pool of an even number of blocks, f32 pools of ranks divisible by 8), go through registers;
-  // 512 pairs of 2,048 kept rows of 612 B: COMPACT_WIDE us against 371 us through shared memory.
+  // 512 pairs of 2,048 kept rows of 612 B: 251 us against 371 us through shared memory.
   const uint32_t pieces = a.row_a / 32 + (a.row_b % 32 ? 0u : a.row_b / 32);
-  if (a.row_a % 32 == 0 && a.row_b % 4 == 0 && pieces <= WIDE * CT) {
+  if (a.row_a % 32 == 0 && a.row_b % 4 == 0 && pieces <= WIDE * CT && a.row_a <= 65536 && a.row_b <= 65536) {
     a.tile = WIDE * CT / pieces;
     if (a.row_b % 32 && a.tile > WORDS * CT / (a.row_b / 4)) a.tile = WORDS * CT / (a.row_b / 4);
     if (a.tile > REG_TILE) a.tile = REG_TILE;

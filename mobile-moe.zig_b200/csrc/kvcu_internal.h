@@ -112,9 +112,9 @@ int kvcu_current_sm_count();
     if (_rc) return _rc; \
   } while (0)
 
-// Dynamic shared memory the eviction kernels may ask for (192 KB: 48k keys of a
-// row; their static arrays take up to 17 KB more of an SM's 227 KB).
-#define KVCU_EVICT_SMEM 196608
+// Dynamic shared memory the eviction kernels may ask for (184 KB: 46k keys of a
+// row; their static arrays take up to 33 KB more of an SM's 227 KB).
+#define KVCU_EVICT_SMEM 188416
 
 // ---- kernel launchers (kvcu_kernels.cu) ----
 int kvcu_launch_append(kvcu_pool* p, uint32_t layer, uint32_t n_rows, const float* latent,
