@@ -232,6 +232,13 @@ int kvcu_mla_decode_lse(kvcu_decode_ws* ws, kvcu_pool* pool, uint32_t layer, uin
 int kvcu_mla_prepare(kvcu_pool* pool, uint32_t n, uint32_t n_heads, uint32_t qk_nope, const float* q,
                      const float* kv_a, const uint32_t* positions, const float* norm_w, float eps,
                      float rope_base, const float* k_b, float* q_abs, float* rows, void* stream);
+/* kvcu_mla_prepare with the rotary frequencies of `rope` (rot_dim = the pool's
+ * rope_dim) at `positions`, which need not be the rows' places in the cache: after
+ * an eviction a token's position is larger than its row's index. */
+struct kvcu_rope;
+int kvcu_mla_prepare_rope(kvcu_pool* pool, uint32_t n, uint32_t n_heads, uint32_t qk_nope, const float* q,
+                          const float* kv_a, const uint32_t* positions, const float* norm_w, float eps,
+                          const struct kvcu_rope* rope, const float* k_b, float* q_abs, float* rows, void* stream);
 int kvcu_mla_finish(kvcu_pool* pool, uint32_t n, uint32_t n_heads, uint32_t v_dim, const float* q_abs,
                     const float* rows, float* latent, const float* lse, float scale, const float* v_b,
                     float* attn, void* stream);
@@ -615,6 +622,47 @@ int kvcache_mla_step_dev(kvcache* c, uint32_t layer, uint32_t n, const uint32_t*
                          const float* norm_w_dev, float eps, float rope_base, const float* k_b_dev,
                          const float* v_b_dev, uint32_t n_heads, uint32_t qk_nope, uint32_t v_dim,
                          float scale, float* attn_dev, void* stream);
+/* ---- a bounded cache (no counterpart in the reference) ----
+ * The step above with the rotary frequencies of `rope` at rope_positions[b] (host;
+ * NULL: the cache positions): in a cache that evicts, a token's position runs on
+ * while its row goes to the next free place.  q_abs_dev [n][H][R+P] and lse_dev
+ * [n][H] (device, each may be NULL) receive the absorbed queries and the
+ * log-sum-exp of the scaled scores over the history and the newest token, what
+ * kvcache_attn_mass_dev takes. */
+int kvcache_mla_step_rope_dev(kvcache* c, uint32_t layer, uint32_t n, const uint32_t* seq_ids,
+                              const uint32_t* positions, const kvcu_rope* rope, const uint32_t* rope_positions,
+                              const float* q_dev, const float* kv_a_dev, const float* norm_w_dev, float eps,
+                              const float* k_b_dev, const float* v_b_dev, uint32_t n_heads, uint32_t qk_nope,
+                              uint32_t v_dim, float scale, float* attn_dev, float* q_abs_dev, float* lse_dev,
+                              void* stream);
+/* kvcache_mla_decode_dev and kvcache_mla_attention_batch_dev that also write the
+ * log-sum-exp of the scaled scores (lse [n][H] / [n_pos][H], device). */
+int kvcache_mla_decode_lse_dev(kvcache* c, uint32_t layer, uint32_t n, const uint32_t* seq_ids, const float* q_dev,
+                               uint32_t n_heads, float scale, float* out_dev, float* lse_dev, void* stream);
+int kvcache_mla_attention_batch_lse_dev(kvcache* c, uint32_t layer, uint32_t seq, uint32_t start_pos, uint32_t n_pos,
+                                        const float* q_dev, uint32_t n_heads, float scale, float* out_dev,
+                                        float* lse_dev, void* stream);
+/* kvcu_attn_mass over whole sequences: entry b's n_q queries are those of the
+ * newest n_q positions of seq_ids[b].  old_lens (host, NULL: all old): sums of
+ * positions >= old_lens[b] start anew.  Every sequence must fit mass_stride.  Right
+ * after a step of the same batch it runs on the step's plan. */
+int kvcache_attn_mass_dev(kvcache* c, uint32_t layer, uint32_t n, const uint32_t* seq_ids, uint32_t n_q,
+                          const float* q_dev, const float* lse_dev, uint32_t n_heads, float scale, float decay,
+                          const uint32_t* old_lens, float* mass_dev, uint64_t mass_stride, void* stream);
+/* Bring every listed sequence (each once) that is longer than `budget` down to
+ * budget rows in all layers: per layer the first n_sink, the last n_recent and
+ * the rows of the largest mass between (kvcu_evict_select, kvcu_evict_compact),
+ * mass [n_layers][n][mass_stride] moved along; its length becomes budget and the
+ * blocks behind return to the pool, as after a truncate.  Blocks held elsewhere
+ * (a shared prefix, a running save) are copied before rows move into them
+ * (KVCU_ERR_OUT_OF_BLOCKS where none is free; nothing is evicted then), and
+ * rewritten blocks leave the prefix cache.  keep_dev (device, may be NULL)
+ * receives the kept positions [n_layers][n][budget].  Call it between steps,
+ * when every layer holds the sequences' rows; it must be ordered after the
+ * calls that read them and before those that reuse the blocks (one stream). */
+int kvcache_evict_dev(kvcache* c, uint32_t n, const uint32_t* seq_ids, uint32_t budget, uint32_t n_sink,
+                      uint32_t n_recent, float* mass_dev, uint64_t mass_layer_stride, uint64_t mass_stride,
+                      uint32_t* keep_dev, void* stream);
 /* Device variant: q/out device pointers, no host copies; plans once per step
  * (a plan is reused until a sequence length or the batch changes). */
 int kvcache_mla_decode_dev(kvcache* c, uint32_t layer, uint32_t n, const uint32_t* seq_ids,

@@ -220,6 +220,12 @@ struct kvcache {
   size_t d_step_cap = 0;
   uint32_t* d_stepu = nullptr;
   size_t d_stepu_cap = 0;
+  // a bounded cache: ids, old lengths, counts and keep lists on the device, in use
+  // until `bound_done`; their uploads
+  uint32_t* d_bound = nullptr;
+  size_t d_bound_cap = 0;
+  HostStage up_bound;
+  cudaEvent_t bound_done = nullptr;
   // decode
   kvcu_decode_ws* ws = nullptr;
   uint32_t ws_batch = 0, ws_heads = 0, ws_layers = 0;
@@ -595,11 +601,10 @@ int ensure_ws(kvcache* c, uint32_t n, uint32_t n_heads, uint32_t n_layers = 1) {
   return KVCU_OK;
 }
 
-// Decode layers [layer, layer + n_layers) of a batch (q / out of layer+i at
-// + i * the stride, floats); n_layers > 1 runs as one multi-layer launch.
-int decode_impl(kvcache* c, uint32_t layer, uint32_t n, const uint32_t* seq_ids, const float* q_dev,
-                uint32_t n_heads, float scale, float* out_dev, cudaStream_t st, uint32_t n_layers = 1,
-                uint64_t q_lstride = 0, uint64_t out_lstride = 0) {
+// The workspace, tables, lengths and plan of a batch (checked first) for layers
+// [layer, layer + n_layers); `launches` is set to those it took.
+int plan_batch(kvcache* c, uint32_t layer, uint32_t n, const uint32_t* seq_ids, uint32_t n_heads, cudaStream_t st,
+               uint32_t n_layers, uint32_t* launches_out) {
   if (n_layers == 0 || layer >= c->n_layers || n_layers > c->n_layers - layer) {
     kvcu_set_error("LayerOutOfBounds: layers [%u, %u + %u) of %u", layer, layer, n_layers, c->n_layers);
     return KVCU_ERR_LAYER_OOB;
@@ -646,7 +651,23 @@ int decode_impl(kvcache* c, uint32_t layer, uint32_t n, const uint32_t* seq_ids,
     c->plan_tokens = tokens;
     c->plan_layers = plan_layers;
   }
-  if (n_layers == 1)
+  *launches_out = launches;
+  return KVCU_OK;
+}
+
+// Decode layers [layer, layer + n_layers) of a batch (q / out of layer+i at
+// + i * the stride, floats); n_layers > 1 runs as one multi-layer launch.  lse
+// (nullable): the log-sum-exp of a one-layer decode.
+int decode_impl(kvcache* c, uint32_t layer, uint32_t n, const uint32_t* seq_ids, const float* q_dev,
+                uint32_t n_heads, float scale, float* out_dev, cudaStream_t st, uint32_t n_layers = 1,
+                uint64_t q_lstride = 0, uint64_t out_lstride = 0, float* lse = nullptr) {
+  uint32_t launches = 0;
+  int rc = plan_batch(c, layer, n, seq_ids, n_heads, st, n_layers, &launches);
+  if (rc) return rc;
+  if (n_layers == 1 && lse)
+    rc = kvcu_mla_decode_lse(c->ws, c->pool, layer, n, c->d_seq_ids, (uint32_t)c->seqs.size(), c->d_toff,
+                             c->d_tables, c->d_lens, q_dev, n_heads, scale, out_dev, lse, st);
+  else if (n_layers == 1)
     rc = kvcu_mla_decode(c->ws, c->pool, layer, n, c->d_seq_ids, (uint32_t)c->seqs.size(), c->d_toff,
                          c->d_tables, c->d_lens, q_dev, n_heads, scale, out_dev, st);
   else
@@ -662,7 +683,8 @@ int decode_impl(kvcache* c, uint32_t layer, uint32_t n, const uint32_t* seq_ids,
 // src/inference.zig:771-877): query i is position start_pos + i and attends
 // positions [0, start_pos + i].  Stream-ordered on `st`.
 int attention_batch_impl(kvcache* c, uint32_t layer, uint32_t seq, uint32_t start_pos, uint32_t n_pos,
-                         const float* q_dev, uint32_t n_heads, float scale, float* out_dev, cudaStream_t st) {
+                         const float* q_dev, uint32_t n_heads, float scale, float* out_dev, cudaStream_t st,
+                         float* lse = nullptr) {
   if (layer >= c->n_layers) {
     kvcu_set_error("LayerOutOfBounds: layer %u >= %u", layer, c->n_layers);
     return KVCU_ERR_LAYER_OOB;
@@ -693,12 +715,129 @@ int attention_batch_impl(kvcache* c, uint32_t layer, uint32_t seq, uint32_t star
   ++c->plan_serial;
   c->plan_epoch = ~0ull;  // the cached decode plan no longer matches the workspace
   c->plan_ids.clear();
-  if (!rc)
+  if (!rc && lse)
+    rc = kvcu_mla_decode_lse(c->ws, c->pool, layer, n_pos, c->d_stepu, n_seqs, c->d_toff, c->d_tables, c->d_lens, q_dev,
+                             n_heads, scale, out_dev, lse, st);
+  else if (!rc)
     rc = kvcu_mla_decode(c->ws, c->pool, layer, n_pos, c->d_stepu, n_seqs, c->d_toff, c->d_tables, c->d_lens, q_dev,
                          n_heads, scale, out_dev, st);
   if (rc) return rc;
   c->last_launches = 1 + kvcu_decode_last_launches(c->ws);
   return KVCU_OK;
+}
+
+// The MLA step.  rope (nullable): its rotary positions by these frequencies at
+// rope_positions (host; nullable: the cache positions), else plain ones of
+// rope_base at the cache positions.  q_abs_out / lse_out (device, nullable): the
+// absorbed queries, and the log-sum-exp over the history and the newest token.
+int step_impl(kvcache* c, uint32_t layer, uint32_t n, const uint32_t* seq_ids, const uint32_t* positions,
+              const kvcu_rope* rope, const uint32_t* rope_positions, const float* q_dev, const float* kv_a_dev,
+              const float* norm_w_dev, float eps, float rope_base, const float* k_b_dev, const float* v_b_dev,
+              uint32_t n_heads, uint32_t qk_nope, uint32_t v_dim, float scale, float* attn_dev, float* q_abs_out,
+              float* lse_out, void* stream) {
+  if (!c || (n && (!seq_ids || !positions || !q_dev || !kv_a_dev || !norm_w_dev || !k_b_dev ||
+                   !v_b_dev || !attn_dev)))
+    return KVCU_ERR_INVALID_ARG;
+  if (!n) return KVCU_OK;
+  DevScope d(c->device);
+  const cudaStream_t st = (cudaStream_t)stream;
+  int rc = validate_positions(c, layer, n, seq_ids, positions);
+  if (!rc) rc = cow_for_write(c, n, seq_ids, positions, st);
+  if (rc) return rc;
+  const uint32_t R = c->kv_rank, Wd = c->row_width(), n_seqs = (uint32_t)c->seqs.size();
+  // scratch: q_abs [n][H][W], rows [n][W], latent [n][H][R], lse [n][H], merge weights [n][H][3]
+  const size_t q_abs_n = (size_t)n * n_heads * Wd, rows_n = (size_t)n * Wd, lat_n = (size_t)n * n_heads * R;
+  rc = ensure_dev(&c->d_step, &c->d_step_cap, q_abs_n + rows_n + lat_n + (size_t)n * n_heads * 4);
+  if (!rc) rc = ensure_dev(&c->d_stepu, &c->d_stepu_cap, 3 * (size_t)n + n_seqs);
+  if (!rc) rc = sync_tables(c, st);
+  if (!rc) rc = sync_lens(c, st);
+  if (!rc) rc = ensure_ws(c, n, n_heads);
+  if (rc) return rc;
+  float* q_abs = q_abs_out ? q_abs_out : c->d_step;
+  float* rows = c->d_step + q_abs_n;
+  float* latent = rows + rows_n;
+  float* lse = latent + lat_n;
+  float* mrg_w = lse + (size_t)n * n_heads;  // [n][H][3] merge weights
+  uint32_t* d_ids = c->d_stepu;
+  uint32_t* d_pos = d_ids + n;
+  uint32_t* d_hist = d_pos + n;
+  uint32_t* d_rot = d_hist + n_seqs;
+  // the decode covers each entry's history, positions < pos (the newest token
+  // is merged by kvcu_mla_finish as the reference treats it)
+  std::vector<uint32_t> hist(n_seqs, 0);
+  std::vector<char> seen(n_seqs, 0);
+  for (uint32_t b = 0; b < n; ++b) {
+    if (seen[seq_ids[b]]) {
+      kvcu_set_error("kvcache_mla_step_dev: sequence %u appears twice in the batch", seq_ids[b]);
+      return KVCU_ERR_INVALID_ARG;
+    }
+    seen[seq_ids[b]] = 1;
+    hist[seq_ids[b]] = positions[b];
+  }
+  // d_ids belong to the kept plan: other ones void it, also where this step fails below
+  if (c->mla_plan_ids.size() != n || !std::equal(c->mla_plan_ids.begin(), c->mla_plan_ids.end(), seq_ids))
+    c->mla_plan_serial = ~0ull;
+  KVCU_CUDA(cudaMemcpyAsync(d_ids, seq_ids, (size_t)n * 4, cudaMemcpyHostToDevice, st));
+  KVCU_CUDA(cudaMemcpyAsync(d_pos, positions, (size_t)n * 4, cudaMemcpyHostToDevice, st));
+  KVCU_CUDA(cudaMemcpyAsync(d_hist, hist.data(), (size_t)n_seqs * 4, cudaMemcpyHostToDevice, st));
+  if (rope && rope_positions)
+    KVCU_CUDA(cudaMemcpyAsync(d_rot, rope_positions, (size_t)n * 4, cudaMemcpyHostToDevice, st));
+  rc = rope ? kvcu_mla_prepare_rope(c->pool, n, n_heads, qk_nope, q_dev, kv_a_dev, rope_positions ? d_rot : d_pos,
+                                    norm_w_dev, eps, rope, k_b_dev, q_abs, rows, st)
+            : kvcu_mla_prepare(c->pool, n, n_heads, qk_nope, q_dev, kv_a_dev, d_pos, norm_w_dev, eps, rope_base,
+                               k_b_dev, q_abs, rows, st);
+  if (!rc)
+    rc = kvcu_append(c->pool, layer, n, rows, Wd, rows + R, Wd, d_ids, d_pos, n_seqs, c->d_toff, c->d_tables,
+                     c->d_lens, st);
+  if (rc) return rc;
+  bump_lens(c, n, seq_ids, positions);  // the append kernel advanced d_lens identically
+  // The plan depends only on the batch and its history lengths, which the
+  // layers of one step share: the first layer plans, the others reuse it.
+  const bool same_plan = c->mla_plan_serial == c->plan_serial && c->mla_plan_ids.size() == n &&
+                         std::equal(c->mla_plan_ids.begin(), c->mla_plan_ids.end(), seq_ids) &&
+                         std::equal(c->mla_plan_hist.begin(), c->mla_plan_hist.end(), positions);
+  if (!same_plan) {
+    rc = kvcu_decode_plan(c->ws, c->pool, n, d_ids, n_seqs, d_hist, st);
+    c->plan_epoch = ~0ull;  // the cached decode plan no longer matches the workspace
+    c->mla_plan_serial = rc ? ~0ull : ++c->plan_serial;
+    c->mla_plan_ids.assign(seq_ids, seq_ids + n);
+    c->mla_plan_hist.assign(positions, positions + n);
+  }
+  if (!rc)
+    rc = kvcu_mla_decode_lse(c->ws, c->pool, layer, n, d_ids, n_seqs, c->d_toff, c->d_tables, d_hist, q_abs,
+                             n_heads, scale, latent, lse, st);
+  if (!rc)
+    rc = kvcu_mla_finish_fused(c->pool, n, n_heads, v_dim, q_abs, rows, latent, lse, mrg_w, scale, v_b_dev, attn_dev,
+                               st, lse_out);
+  if (rc) return rc;
+  // rows, rotary positions of their own, gemm (prepare) + append + plan + decode +
+  // merge, gemm (finish). The host arrays above are pageable: each cudaMemcpyAsync
+  // returned only after staging them, so they may go out of scope now.
+  c->last_launches = 2 + (rope ? 1 : 0) + 1 + (same_plan ? 0 : 1) + kvcu_decode_last_launches(c->ws) + 2;
+  return KVCU_OK;
+}
+
+// No exception leaves a C entry point.
+template <typename F>
+int guarded(const char* what, F f) {
+  try {
+    return f();
+  } catch (const std::bad_alloc&) {
+    kvcu_set_error("%s: out of host memory", what);
+    return KVCU_ERR_NO_MEMORY;
+  } catch (...) {
+    kvcu_set_error("%s: unexpected failure", what);
+    return KVCU_ERR_INVALID_ARG;
+  }
+}
+
+// The bounded cache's device scratch: `words` of it for a call on `st`, after the
+// call before (on whichever stream) is through with it.
+int bound_acquire(kvcache* c, size_t words, size_t staged, cudaStream_t st) {
+  if (!c->bound_done) KVCU_CUDA(cudaEventCreateWithFlags(&c->bound_done, cudaEventDisableTiming));
+  else KVCU_CUDA(cudaStreamWaitEvent(st, c->bound_done, 0));
+  const int rc = ensure_dev(&c->d_bound, &c->d_bound_cap, words);
+  return rc ? rc : stage_acquire(c->up_bound, staged);
 }
 
 }  // namespace
@@ -712,6 +851,16 @@ int kvcache_mla_attention_batch_dev(kvcache* c, uint32_t layer, uint32_t seq, ui
   if (!n_pos) return KVCU_OK;
   DevScope d(c->device);
   return attention_batch_impl(c, layer, seq, start_pos, n_pos, q_dev, n_heads, scale, out_dev, (cudaStream_t)stream);
+}
+
+int kvcache_mla_attention_batch_lse_dev(kvcache* c, uint32_t layer, uint32_t seq, uint32_t start_pos, uint32_t n_pos,
+                                        const float* q_dev, uint32_t n_heads, float scale, float* out_dev,
+                                        float* lse_dev, void* stream) {
+  if (!c || (n_pos && (!q_dev || !out_dev || !lse_dev))) return KVCU_ERR_INVALID_ARG;
+  if (!n_pos) return KVCU_OK;
+  DevScope d(c->device);
+  return attention_batch_impl(c, layer, seq, start_pos, n_pos, q_dev, n_heads, scale, out_dev, (cudaStream_t)stream,
+                              lse_dev);
 }
 
 int kvcache_mla_attention_batch(kvcache* c, uint32_t layer, uint32_t seq, uint32_t start_pos, uint32_t n_pos,
@@ -774,6 +923,9 @@ void kvcache_deinit(kvcache* c) {
   stage_free(c->up_tables);
   stage_free(c->up_lens);
   stage_free(c->up_rowidx);
+  if (c->bound_done) cudaEventDestroy(c->bound_done);
+  cudaFree(c->d_bound);
+  stage_free(c->up_bound);
   if (c->stream) cudaStreamDestroy(c->stream);
   delete c;
 }
@@ -1170,78 +1322,157 @@ int kvcache_mla_step_dev(kvcache* c, uint32_t layer, uint32_t n, const uint32_t*
                          const float* norm_w_dev, float eps, float rope_base, const float* k_b_dev,
                          const float* v_b_dev, uint32_t n_heads, uint32_t qk_nope, uint32_t v_dim,
                          float scale, float* attn_dev, void* stream) {
-  if (!c || (n && (!seq_ids || !positions || !q_dev || !kv_a_dev || !norm_w_dev || !k_b_dev ||
-                   !v_b_dev || !attn_dev)))
+  return step_impl(c, layer, n, seq_ids, positions, nullptr, nullptr, q_dev, kv_a_dev, norm_w_dev, eps, rope_base,
+                   k_b_dev, v_b_dev, n_heads, qk_nope, v_dim, scale, attn_dev, nullptr, nullptr, stream);
+}
+
+int kvcache_mla_step_rope_dev(kvcache* c, uint32_t layer, uint32_t n, const uint32_t* seq_ids,
+                              const uint32_t* positions, const kvcu_rope* rope, const uint32_t* rope_positions,
+                              const float* q_dev, const float* kv_a_dev, const float* norm_w_dev, float eps,
+                              const float* k_b_dev, const float* v_b_dev, uint32_t n_heads, uint32_t qk_nope,
+                              uint32_t v_dim, float scale, float* attn_dev, float* q_abs_dev, float* lse_dev,
+                              void* stream) {
+  if (!rope || !c || rope->rot != c->rope_dim) {
+    kvcu_set_error("kvcache_mla_step_rope_dev: rotary part of %u, the cache's has %u", rope ? rope->rot : 0u,
+                   c ? c->rope_dim : 0u);
     return KVCU_ERR_INVALID_ARG;
+  }
+  return guarded("kvcache_mla_step_rope_dev", [&] {
+    return step_impl(c, layer, n, seq_ids, positions, rope, rope_positions, q_dev, kv_a_dev, norm_w_dev, eps, 0.0f,
+                     k_b_dev, v_b_dev, n_heads, qk_nope, v_dim, scale, attn_dev, q_abs_dev, lse_dev, stream);
+  });
+}
+
+int kvcache_mla_decode_lse_dev(kvcache* c, uint32_t layer, uint32_t n, const uint32_t* seq_ids, const float* q_dev,
+                               uint32_t n_heads, float scale, float* out_dev, float* lse_dev, void* stream) {
+  if (!c || (n && (!seq_ids || !q_dev || !out_dev || !lse_dev))) return KVCU_ERR_INVALID_ARG;
+  if (!n) return KVCU_OK;
+  DevScope d(c->device);
+  return guarded("kvcache_mla_decode_lse_dev", [&] {
+    return decode_impl(c, layer, n, seq_ids, q_dev, n_heads, scale, out_dev, (cudaStream_t)stream, 1, 0, 0, lse_dev);
+  });
+}
+
+int kvcache_attn_mass_dev(kvcache* c, uint32_t layer, uint32_t n, const uint32_t* seq_ids, uint32_t n_q,
+                          const float* q_dev, const float* lse_dev, uint32_t n_heads, float scale, float decay,
+                          const uint32_t* old_lens, float* mass_dev, uint64_t mass_stride, void* stream) {
+  if (!c || (n && (!seq_ids || !q_dev || !lse_dev || !mass_dev))) return KVCU_ERR_INVALID_ARG;
   if (!n) return KVCU_OK;
   DevScope d(c->device);
   const cudaStream_t st = (cudaStream_t)stream;
-  int rc = validate_positions(c, layer, n, seq_ids, positions);
-  if (!rc) rc = cow_for_write(c, n, seq_ids, positions, st);
-  if (rc) return rc;
-  const uint32_t R = c->kv_rank, Wd = c->row_width(), n_seqs = (uint32_t)c->seqs.size();
-  // scratch: q_abs [n][H][W], rows [n][W], latent [n][H][R], lse [n][H], merge weights [n][H][3]
-  const size_t q_abs_n = (size_t)n * n_heads * Wd, rows_n = (size_t)n * Wd, lat_n = (size_t)n * n_heads * R;
-  rc = ensure_dev(&c->d_step, &c->d_step_cap, q_abs_n + rows_n + lat_n + (size_t)n * n_heads * 4);
-  if (!rc) rc = ensure_dev(&c->d_stepu, &c->d_stepu_cap, 2 * (size_t)n + n_seqs);
-  if (!rc) rc = sync_tables(c, st);
-  if (!rc) rc = sync_lens(c, st);
-  if (!rc) rc = ensure_ws(c, n, n_heads);
-  if (rc) return rc;
-  float* q_abs = c->d_step;
-  float* rows = q_abs + q_abs_n;
-  float* latent = rows + rows_n;
-  float* lse = latent + lat_n;
-  float* mrg_w = lse + (size_t)n * n_heads;  // [n][H][3] merge weights
-  uint32_t* d_ids = c->d_stepu;
-  uint32_t* d_pos = d_ids + n;
-  uint32_t* d_hist = d_pos + n;
-  // the decode covers each entry's history, positions < pos (the newest token
-  // is merged by kvcu_mla_finish as the reference treats it)
-  std::vector<uint32_t> hist(n_seqs, 0);
-  std::vector<char> seen(n_seqs, 0);
-  for (uint32_t b = 0; b < n; ++b) {
-    if (seen[seq_ids[b]]) {
-      kvcu_set_error("kvcache_mla_step_dev: sequence %u appears twice in the batch", seq_ids[b]);
-      return KVCU_ERR_INVALID_ARG;
+  return guarded("kvcache_attn_mass_dev", [&]() -> int {
+    for (uint32_t b = 0; b < n; ++b)
+      if (seq_ids[b] < c->seqs.size() && c->seqs[seq_ids[b]].len > mass_stride) {
+        kvcu_set_error("kvcache_attn_mass_dev: sequence %u holds %u positions, a row of sums %llu", seq_ids[b],
+                       c->seqs[seq_ids[b]].len, (unsigned long long)mass_stride);
+        return KVCU_ERR_INVALID_ARG;
+      }
+    // The plan of the step that has just appended these sequences' newest rows serves
+    // as it is (its open-ended items take the row in); else that of a decode.
+    const uint32_t* ids = c->d_stepu;
+    uint32_t launches = 0;
+    bool step_plan = c->ws && c->mla_plan_serial == c->plan_serial && c->mla_plan_ids.size() == n &&
+                     std::equal(c->mla_plan_ids.begin(), c->mla_plan_ids.end(), seq_ids);
+    for (uint32_t b = 0; step_plan && b < n; ++b) step_plan = c->seqs[seq_ids[b]].len >= c->mla_plan_hist[b];
+    int rc = KVCU_OK;
+    if (step_plan) {
+      rc = sync_tables(c, st);
+      if (!rc) rc = sync_lens(c, st);
+    } else {
+      rc = plan_batch(c, layer, n, seq_ids, n_heads, st, 1, &launches);
+      ids = c->d_seq_ids;
     }
-    seen[seq_ids[b]] = 1;
-    hist[seq_ids[b]] = positions[b];
+    if (!rc && old_lens) rc = bound_acquire(c, n, n, st);
+    if (rc) return rc;
+    if (old_lens) {
+      memcpy(c->up_bound.p, old_lens, (size_t)n * 4);
+      rc = stage_upload(c->up_bound, c->d_bound, n, st);
+      if (rc) return rc;
+    }
+    rc = kvcu_attn_mass(c->ws, c->pool, layer, n, ids, (uint32_t)c->seqs.size(), c->d_toff, c->d_tables,
+                        c->d_lens, n_q, q_dev, lse_dev, n_heads, scale, decay, old_lens ? c->d_bound : nullptr,
+                        mass_dev, mass_stride, st);
+    if (old_lens) KVCU_CUDA(cudaEventRecord(c->bound_done, st));
+    if (rc) return rc;
+    c->last_launches = launches + 1;
+    return KVCU_OK;
+  });
+}
+
+int kvcache_evict_dev(kvcache* c, uint32_t n, const uint32_t* seq_ids, uint32_t budget, uint32_t n_sink,
+                      uint32_t n_recent, float* mass_dev, uint64_t mass_layer_stride, uint64_t mass_stride,
+                      uint32_t* keep_dev, void* stream) {
+  if (!c || (n && (!seq_ids || !mass_dev))) return KVCU_ERR_INVALID_ARG;
+  if (budget == 0 || (uint64_t)n_sink + n_recent > budget || budget == KVCU_NO_POSITION) {
+    kvcu_set_error("kvcache_evict_dev: budget %u with %u first and %u last positions", budget, n_sink, n_recent);
+    return KVCU_ERR_INVALID_ARG;
   }
-  KVCU_CUDA(cudaMemcpyAsync(d_ids, seq_ids, (size_t)n * 4, cudaMemcpyHostToDevice, st));
-  KVCU_CUDA(cudaMemcpyAsync(d_pos, positions, (size_t)n * 4, cudaMemcpyHostToDevice, st));
-  KVCU_CUDA(cudaMemcpyAsync(d_hist, hist.data(), (size_t)n_seqs * 4, cudaMemcpyHostToDevice, st));
-  rc = kvcu_mla_prepare(c->pool, n, n_heads, qk_nope, q_dev, kv_a_dev, d_pos, norm_w_dev, eps, rope_base,
-                        k_b_dev, q_abs, rows, st);
-  if (!rc)
-    rc = kvcu_append(c->pool, layer, n, rows, Wd, rows + R, Wd, d_ids, d_pos, n_seqs, c->d_toff, c->d_tables,
-                     c->d_lens, st);
-  if (rc) return rc;
-  bump_lens(c, n, seq_ids, positions);  // the append kernel advanced d_lens identically
-  // The plan depends only on the batch and its history lengths, which the
-  // layers of one step share: the first layer plans, the others reuse it.
-  const bool same_plan = c->mla_plan_serial == c->plan_serial && c->mla_plan_ids.size() == n &&
-                         std::equal(c->mla_plan_ids.begin(), c->mla_plan_ids.end(), seq_ids) &&
-                         std::equal(c->mla_plan_hist.begin(), c->mla_plan_hist.end(), positions);
-  if (!same_plan) {
-    rc = kvcu_decode_plan(c->ws, c->pool, n, d_ids, n_seqs, d_hist, st);
-    c->plan_epoch = ~0ull;  // the cached decode plan no longer matches the workspace
-    c->mla_plan_serial = rc ? ~0ull : ++c->plan_serial;
-    c->mla_plan_ids.assign(seq_ids, seq_ids + n);
-    c->mla_plan_hist.assign(positions, positions + n);
-  }
-  if (!rc)
-    rc = kvcu_mla_decode_lse(c->ws, c->pool, layer, n, d_ids, n_seqs, c->d_toff, c->d_tables, d_hist, q_abs,
-                             n_heads, scale, latent, lse, st);
-  if (!rc)
-    rc = kvcu_mla_finish_fused(c->pool, n, n_heads, v_dim, q_abs, rows, latent, lse, mrg_w, scale, v_b_dev, attn_dev,
-                               st);
-  if (rc) return rc;
-  // rows, gemm (prepare) + append + plan + decode + merge, gemm (finish). The
-  // three host arrays above are pageable: each cudaMemcpyAsync returned only
-  // after staging them, so they may go out of scope now.
-  c->last_launches = 2 + 1 + (same_plan ? 0 : 1) + kvcu_decode_last_launches(c->ws) + 2;
-  return KVCU_OK;
+  c->last_launches = 0;
+  if (!n) return KVCU_OK;
+  DevScope d(c->device);
+  const cudaStream_t st = (cudaStream_t)stream;
+  return guarded("kvcache_evict_dev", [&]() -> int {
+    std::vector<char> seen(c->seqs.size(), 0);
+    bool any = false;
+    for (uint32_t b = 0; b < n; ++b) {
+      const uint32_t s = seq_ids[b];
+      if (s >= c->seqs.size() || seen[s]) {
+        kvcu_set_error("kvcache_evict_dev: sequence %u %s", s, s >= c->seqs.size() ? "does not exist" : "appears twice");
+        return KVCU_ERR_INVALID_ARG;
+      }
+      seen[s] = 1;
+      if (c->seqs[s].len > mass_stride) {
+        kvcu_set_error("kvcache_evict_dev: sequence %u holds %u positions, a row of sums %llu", s, c->seqs[s].len,
+                       (unsigned long long)mass_stride);
+        return KVCU_ERR_INVALID_ARG;
+      }
+      any = any || c->seqs[s].len > budget;
+    }
+    if (!any && !keep_dev) return KVCU_OK;
+    // The blocks that rows move into: copied first where another sequence or a
+    // running save holds them too, and no longer what their prefix hash says.
+    // Blocks wholly inside the first n_sink positions keep their rows.
+    for (uint32_t b = 0; b < n; ++b) {
+      Seq& q = c->seqs[seq_ids[b]];
+      if (q.len <= budget) continue;
+      const uint32_t end = (uint32_t)(((uint64_t)budget + c->block_size - 1) / c->block_size);
+      for (uint32_t bi = n_sink / c->block_size; bi < end; ++bi) {
+        const uint32_t pos = bi * c->block_size;
+        const int rc = cow_for_write(c, 1, seq_ids + b, &pos, st);
+        if (rc) return rc;
+        const uint32_t id = q.table[bi];
+        if (c->hash[id] != kNoHash) {
+          auto it = c->hash_map.find(c->hash[id]);
+          if (it != c->hash_map.end() && it->second == id) c->hash_map.erase(it);
+          c->hash[id] = kNoHash;
+        }
+      }
+    }
+    const size_t list = keep_dev ? 0 : (size_t)c->n_layers * n * budget;
+    int rc = bound_acquire(c, 2 * (size_t)n + list, n, st);
+    if (!rc) rc = sync_tables(c, st);
+    if (!rc) rc = sync_lens(c, st);
+    if (rc) return rc;
+    uint32_t* ids = c->d_bound;
+    uint32_t* counts = ids + n;
+    uint32_t* keep = keep_dev ? keep_dev : counts + n;
+    memcpy(c->up_bound.p, seq_ids, (size_t)n * 4);
+    rc = stage_upload(c->up_bound, ids, n, st);
+    const uint32_t n_seqs = (uint32_t)c->seqs.size();
+    if (!rc)
+      rc = kvcu_evict_select(c->pool, c->n_layers, n, ids, n_seqs, c->d_lens, budget, n_sink, n_recent, mass_dev,
+                             mass_layer_stride, mass_stride, keep, (uint64_t)n * budget, budget, counts, st);
+    if (!rc)
+      rc = kvcu_evict_compact(c->pool, 0, c->n_layers, n, ids, n_seqs, c->d_toff, c->d_tables, keep,
+                              (uint64_t)n * budget, budget, counts, mass_dev, mass_layer_stride, mass_stride, c->d_lens,
+                              st);
+    KVCU_CUDA(cudaEventRecord(c->bound_done, st));
+    if (rc) return rc;
+    for (uint32_t b = 0; b < n; ++b)
+      if (c->seqs[seq_ids[b]].len > budget) seq_truncate(c, seq_ids[b], budget);
+    c->last_launches = 2;
+    return KVCU_OK;
+  });
 }
 
 uint32_t kvcache_last_launches(const kvcache* c) { return c ? c->last_launches : 0; }

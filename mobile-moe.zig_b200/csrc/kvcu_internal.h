@@ -173,10 +173,11 @@ int kvcu_launch_head_gemm_tc(bool trans_b, uint32_t heads, uint32_t M, uint32_t 
                              uint32_t ldc, uint64_t c_hs, uint32_t* status, cudaStream_t st,
                              const kvcu_gemm_merge* mrg = nullptr);
 // kvcu_mla_finish with scratch w [n][n_heads][3] for the merge weights, so the
-// v_b GEMM merges while it loads (kvcu_mla.cu); stream-ordered on st.
+// v_b GEMM merges while it loads (kvcu_mla.cu); stream-ordered on st.  lse_out
+// (nullable) [n][n_heads]: the log-sum-exp with the newest token.
 int kvcu_mla_finish_fused(kvcu_pool* pool, uint32_t n, uint32_t n_heads, uint32_t v_dim, const float* q_abs,
                           const float* rows, float* latent, const float* lse, float* w, float scale,
-                          const float* v_b, float* attn, cudaStream_t st);
+                          const float* v_b, float* attn, cudaStream_t st, float* lse_out = nullptr);
 // ---- allocation-free decode (kvcu_noalloc.cu) ----
 // Resolve (and so reserve) the fixed decode scratch on `device`, which must be
 // current; kvcu_init calls it.

@@ -39,7 +39,9 @@ constexpr int ROWS_THREADS = 256;
 
 // One CTA per batch entry: RMSNorm of the latent, RoPE of k_pe and of every
 // head's q_rope. Multiplies and adds are _rn so that no FMA contraction
-// changes a rounding against the reference's f32 arithmetic.
+// changes a rounding against the reference's f32 arithmetic.  Without ROPE the
+// rotary parts are left to kvcu_rope_apply.
+template <bool ROPE>
 __global__ void __launch_bounds__(ROWS_THREADS)
     k_mla_rows(uint32_t H, uint32_t qk_nope, uint32_t R, uint32_t P, const float* __restrict__ q,
                const float* __restrict__ kv_a, const uint32_t* __restrict__ pos,
@@ -63,6 +65,7 @@ __global__ void __launch_bounds__(ROWS_THREADS)
   // ss / n + eps, inv = 1 / sqrt(.), out = x * inv * w (math.zig:25-34)
   const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(tot, (float)R), eps)));
   for (uint32_t i = tid; i < R; i += blockDim.x) row[i] = __fmul_rn(__fmul_rn(x[i], inv), norm_w[i]);
+  if constexpr (!ROPE) return;
   // RoPE on pairs (2i, 2i+1), i < P/2 (math.zig:227-238): k_pe, then each head's q_rope
   const float pf = (float)pos[b];
   const uint32_t half = P / 2;
@@ -210,7 +213,7 @@ constexpr int MERGE_THREADS = 128;
 __global__ void __launch_bounds__(MERGE_THREADS)
     k_mla_merge_w(uint32_t H, uint32_t R, uint32_t P, int kpe_q8, const float* __restrict__ q_abs,
                   const float* __restrict__ rows, const float* __restrict__ lse, float scale,
-                  float* __restrict__ w) {
+                  float* __restrict__ w, float* __restrict__ lse_out) {
   extern __shared__ float msh[];  // [R] latent of the newest token, then [P] its k_pe
   kvcu_pdl_wait();     // launched programmatically after the decode's combine
   kvcu_pdl_trigger();  // the v_b product may start its set-up
@@ -256,6 +259,7 @@ __global__ void __launch_bounds__(MERGE_THREADS)
       wr[0] = wh;
       wr[1] = wc;
       wr[2] = 1.0f / (wh + wc);
+      if (lse_out) lse_out[(uint64_t)b * H + h] = m + logf(wh + wc);  // of the history and the newest token
     }
   }
 }
@@ -364,11 +368,37 @@ extern "C" int kvcu_mla_prepare(kvcu_pool* pool, uint32_t n, uint32_t n_heads, u
   if (d.rc) return d.rc;
   const uint32_t R = pool->kv_rank, P = pool->rope_dim;
   const cudaStream_t st = (cudaStream_t)stream;
-  int rc = kvcu_check_cuda(kvcu_launch_pdl(k_mla_rows, dim3(n), dim3(ROWS_THREADS), 0, st, n_heads, qk_nope, R, P,
-                                           q, kv_a, positions, norm_w, eps, rope_base, q_abs, rows),
+  int rc = kvcu_check_cuda(kvcu_launch_pdl(k_mla_rows<true>, dim3(n), dim3(ROWS_THREADS), 0, st, n_heads, qk_nope, R,
+                                           P, q, kv_a, positions, norm_w, eps, rope_base, q_abs, rows),
                            "mla rows launch");
   if (rc) return rc;
   // q_abs[b][h][0:R] = q_nope[b][h] (n x qk_nope) x k_b_h (qk_nope x R)
+  return launch_head_gemm<false>(n_heads, n, R, qk_nope, q, n_heads * (qk_nope + P), qk_nope + P, k_b, R,
+                                 (uint64_t)qk_nope * R, q_abs, n_heads * (R + P), R + P, pool->status, st);
+}
+
+extern "C" int kvcu_mla_prepare_rope(kvcu_pool* pool, uint32_t n, uint32_t n_heads, uint32_t qk_nope, const float* q,
+                                     const float* kv_a, const uint32_t* positions, const float* norm_w, float eps,
+                                     const kvcu_rope* rope, const float* k_b, float* q_abs, float* rows, void* stream) {
+  if (!valid_dims(pool, n_heads, qk_nope) || !rope || rope->rot != pool->rope_dim) {
+    kvcu_set_error("kvcu_mla_prepare_rope: unsupported n_heads %u / qk_nope %u / pool dims, or rotated part %u of %u",
+                   n_heads, qk_nope, rope ? rope->rot : 0u, pool ? pool->rope_dim : 0u);
+    return KVCU_ERR_INVALID_ARG;
+  }
+  if (!n) return KVCU_OK;
+  if (!q || !kv_a || !positions || !norm_w || !k_b || !q_abs || !rows) return KVCU_ERR_INVALID_ARG;
+  DevScope d(pool->device);
+  if (d.rc) return d.rc;
+  const uint32_t R = pool->kv_rank, P = pool->rope_dim;
+  const cudaStream_t st = (cudaStream_t)stream;
+  int rc = kvcu_check_cuda(kvcu_launch_pdl(k_mla_rows<false>, dim3(n), dim3(ROWS_THREADS), 0, st, n_heads, qk_nope, R,
+                                           P, q, kv_a, positions, norm_w, eps, 0.0f, q_abs, rows),
+                           "mla rows launch");
+  if (rc) return rc;
+  rc = kvcu_rope_apply(rope, pool->device, KVCU_DTYPE_F32, 0, n, positions, q + qk_nope, n_heads,
+                       (uint64_t)n_heads * (qk_nope + P), qk_nope + P, q_abs + R, (uint64_t)n_heads * (R + P), R + P,
+                       kv_a + R, 1, R + P, P, rows + R, R + P, P, stream);
+  if (rc) return rc;
   return launch_head_gemm<false>(n_heads, n, R, qk_nope, q, n_heads * (qk_nope + P), qk_nope + P, k_b, R,
                                  (uint64_t)qk_nope * R, q_abs, n_heads * (R + P), R + P, pool->status, st);
 }
@@ -401,7 +431,7 @@ extern "C" int kvcu_mla_finish(kvcu_pool* pool, uint32_t n, uint32_t n_heads, ui
 // the tensor-core kernel does not fit the shapes.
 int kvcu_mla_finish_fused(kvcu_pool* pool, uint32_t n, uint32_t n_heads, uint32_t v_dim, const float* q_abs,
                           const float* rows, float* latent, const float* lse, float* w, float scale,
-                          const float* v_b, float* attn, cudaStream_t st) {
+                          const float* v_b, float* attn, cudaStream_t st, float* lse_out) {
   if (!valid_dims(pool, n_heads, v_dim)) {
     kvcu_set_error("kvcu_mla_finish: unsupported n_heads %u / v_dim %u / pool dims", n_heads, v_dim);
     return KVCU_ERR_INVALID_ARG;
@@ -411,10 +441,15 @@ int kvcu_mla_finish_fused(kvcu_pool* pool, uint32_t n, uint32_t n_heads, uint32_
   DevScope d(pool->device);
   if (d.rc) return d.rc;
   const uint32_t R = pool->kv_rank, P = pool->rope_dim;
-  if ((uint64_t)(R + P) * sizeof(float) > 48u * 1024u)  // the weights kernel's shared latent and k_pe
+  if ((uint64_t)(R + P) * sizeof(float) > 48u * 1024u) {  // the weights kernel's shared latent and k_pe
+    if (lse_out) {
+      kvcu_set_error("kvcu_mla_finish: no log-sum-exp for rows of %u elements", R + P);
+      return KVCU_ERR_UNSUPPORTED;
+    }
     return kvcu_mla_finish(pool, n, n_heads, v_dim, q_abs, rows, latent, lse, scale, v_b, attn, st);
+  }
   int rc = kvcu_check_cuda(kvcu_launch_pdl(k_mla_merge_w, dim3(n), dim3(MERGE_THREADS), (R + P) * sizeof(float), st,
-                                           n_heads, R, P, pool->quantized ? 1 : 0, q_abs, rows, lse, scale, w),
+                                           n_heads, R, P, pool->quantized ? 1 : 0, q_abs, rows, lse, scale, w, lse_out),
                            "mla merge launch");
   if (rc) return rc;
   const kvcu_gemm_merge mrg{rows, R + P, w};

@@ -102,6 +102,7 @@ _SIGS = {
     "kvcu_decode_ws_test_withhold": (_i32, [_vp, _u32]),
     "kvcu_decode_last_impl": (_i32, [_vp]),
     "kvcu_mla_decode_noalloc": (_i32, [_vp, _u32, _u32, _vp, _u32, _vp, _vp, _vp, _vp, _u32, _f32, _vp, _vp]),
+    "kvcu_mla_prepare_rope": (_i32, [_vp, _u32, _u32, _u32, _vp, _vp, _vp, _vp, _f32, _vp, _vp, _vp, _vp, _vp]),
     "kvcu_attn_mass": (_i32, [_vp, _vp, _u32, _u32, _vp, _u32, _vp, _vp, _vp, _u32, _vp, _vp, _u32, _f32, _f32, _vp,
                               _vp, _u64, _vp]),
     "kvcu_evict_select": (_i32, [_vp, _u32, _u32, _vp, _u32, _vp, _u32, _u32, _u32, _vp, _u64, _u64, _vp, _u64, _u64,
@@ -164,6 +165,12 @@ _SIGS = {
     "kvcache_append_decode_layers": (_i32, [_vp, _u32, _u32, _u32, _vp, _vp, _vp, _vp, _u32, _f32, _vp]),
     "kvcache_mla_step_dev": (_i32, [_vp, _u32, _u32, _vp, _vp, _vp, _vp, _vp, _f32, _f32, _vp, _vp, _u32,
                                     _u32, _u32, _f32, _vp, _vp]),
+    "kvcache_mla_step_rope_dev": (_i32, [_vp, _u32, _u32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _f32, _vp, _vp, _u32, _u32,
+                                         _u32, _f32, _vp, _vp, _vp, _vp]),
+    "kvcache_mla_decode_lse_dev": (_i32, [_vp, _u32, _u32, _vp, _vp, _u32, _f32, _vp, _vp, _vp]),
+    "kvcache_mla_attention_batch_lse_dev": (_i32, [_vp, _u32, _u32, _u32, _u32, _vp, _u32, _f32, _vp, _vp, _vp]),
+    "kvcache_attn_mass_dev": (_i32, [_vp, _u32, _u32, _vp, _u32, _vp, _vp, _u32, _f32, _f32, _vp, _vp, _u64, _vp]),
+    "kvcache_evict_dev": (_i32, [_vp, _u32, _vp, _u32, _u32, _u32, _vp, _u64, _u64, _vp, _vp]),
     "kvcache_last_launches": (_u32, [_vp]),
     "kvcache_last_decode_mapped": (_i32, [_vp]),
     "kvcache_set_host_io": (_i32, [_vp, _i32]),
@@ -548,40 +555,55 @@ class Rope:
         """Rotate q and / or k, [n][heads][rot_dim] CUDA tensors (any row and head strides; f32, bf16
         or f16), by `positions` (int32 / uint32 [n]), into q_out / k_out (default: in place).
         transpose: the gradient of the rotation."""
-        n, args, first = positions.shape[0], [], None
+        n, args, dtype, dev, rot = positions.shape[0], [], None, positions.get_device(), self.rot_dim
         for x, y in ((q, q_out), (k, k_out)):
             if x is None:
-                args += (None, 0, 0, 0, None, 0, 0)
+                args += _NO_TENSOR
                 continue
-            y = x if y is None else y
-            first = x if first is None else first
-            if x.dim() != 3 or x.shape != y.shape or x.shape[0] != n or x.shape[2] != self.rot_dim:
-                raise ValueError(f"Rope.apply: [{n}][heads][{self.rot_dim}] expected, got {tuple(x.shape)} -> "
-                                 f"{tuple(y.shape)}")
-            xs, ys = x.stride(), y.stride()
-            if xs[2] != 1 or ys[2] != 1 or not x.dtype == y.dtype == first.dtype or not x.is_cuda:
-                raise ValueError("Rope.apply: CUDA tensors of one dtype, contiguous in the last dimension")
-            if not x.device == y.device == positions.device:
-                raise ValueError("Rope.apply: tensors of different devices")
-            args += (x.data_ptr(), x.shape[1], xs[0], xs[1], y.data_ptr(), ys[0], ys[1])
-        if first is None:
+            if y is None:
+                y = x
+            xn, heads, xd = x.shape
+            x0, x1, x2 = x.stride()
+            y0, y1, y2 = y.stride()
+            if dtype is None:
+                dtype = x.dtype
+            if xn != n or xd != rot or (y is not x and y.shape != x.shape):
+                raise ValueError(f"Rope.apply: [{n}][heads][{rot}] expected, got {tuple(x.shape)} -> {tuple(y.shape)}")
+            if x2 != 1 or y2 != 1 or x.dtype is not dtype or y.dtype is not dtype:
+                raise ValueError("Rope.apply: tensors of one dtype, contiguous in the last dimension")
+            if dev < 0 or x.get_device() != dev or y.get_device() != dev:
+                raise ValueError("Rope.apply: CUDA tensors of one device")
+            args += (x.data_ptr(), heads, x0, x1, y.data_ptr(), y0, y1)
+        if dtype is None:
             return
-        if positions.element_size() != 4 or not positions.is_contiguous():
+        if positions.element_size() != 4 or positions.stride(0) != 1:
             raise ValueError("Rope.apply: positions must be contiguous 32-bit integers")
-        dtype = _dtype_code(first)
-        rc = lib().kvcu_rope_apply(self._h, first.device.index, dtype, 1 if transpose else 0, n, positions.data_ptr(),
-                                   *args, _stream(stream))
+        rc = _rope_apply()(self._h, dev, _dtype_code(dtype), transpose, n, positions.data_ptr(), *args,
+                           0 if stream is None else _stream(stream))
         if rc:
             check(rc, "kvcu_rope_apply")
 
 
-def _dtype_code(t) -> int:
-    import torch
+_NO_TENSOR = (None, 0, 0, 0, None, 0, 0)
+_fns = {}
 
-    codes = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-    if t.dtype not in codes:
-        raise ValueError(f"dtype {t.dtype}: float32, bfloat16 or float16 expected")
-    return codes[t.dtype]
+
+def _rope_apply():
+    fn = _fns.get("rope")
+    if fn is None:
+        fn = _fns["rope"] = lib().kvcu_rope_apply
+    return fn
+
+
+def _dtype_code(dtype) -> int:
+    if not _fns.get("codes"):
+        import torch
+
+        _fns["codes"] = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    code = _fns["codes"].get(dtype)
+    if code is None:
+        raise ValueError(f"dtype {dtype}: float32, bfloat16 or float16 expected")
+    return code
 
 
 # ------------------------------------------------------------------ host mirror
@@ -864,6 +886,65 @@ class KVCache:
         check(lib().kvcache_mla_step_dev(self._h, layer, n, _np_ptr(s), _np_ptr(p), _dptr(q), _dptr(kv_a),
                                          _dptr(norm_w), eps, rope_base, _dptr(k_b), _dptr(v_b), H, qk_nope,
                                          v_dim, scale, _dptr(attn), _stream(stream)), "mla_step_dev")
+
+    # ---- a bounded cache ----
+    def mla_step_rope_dev(self, layer, seq_ids, positions, rope, q, kv_a, norm_w, eps, k_b, v_b, qk_nope, v_dim, scale,
+                          attn, rope_positions=None, q_abs=None, lse=None, stream=None):
+        """mla_step_dev with the rotary frequencies of `rope` (a Rope) at rope_positions (default: the
+        cache positions); q_abs [n][H][R+P] and lse [n][H] (device, optional) receive what attnMass_dev takes."""
+        s = np.ascontiguousarray(seq_ids, np.uint32)
+        p = np.ascontiguousarray(positions, np.uint32)
+        rp = None if rope_positions is None else np.ascontiguousarray(rope_positions, np.uint32)
+        n, H = q.shape[0], q.shape[1]
+        if s.size != n or p.size != n or (rp is not None and rp.size != n):
+            raise ValueError(f"mla_step_rope_dev: {n} queries, other numbers of sequences or positions")
+        check(lib().kvcache_mla_step_rope_dev(self._h, layer, n, _np_ptr(s), _np_ptr(p), rope.handle,
+                                              None if rp is None else _np_ptr(rp), _dptr(q), _dptr(kv_a),
+                                              _dptr(norm_w), eps, _dptr(k_b), _dptr(v_b), H, qk_nope, v_dim, scale,
+                                              _dptr(attn), _dptr(q_abs), _dptr(lse), _stream(stream)),
+              "mla_step_rope_dev")
+
+    def mlaDecodeLse_dev(self, layer, seq_ids, q_dev, scale, out_dev, lse_dev, stream=None):
+        """mlaDecode_dev that also writes lse [n][H], the log-sum-exp of the scaled scores."""
+        s = np.ascontiguousarray(seq_ids, np.uint32)
+        n, H = q_dev.shape[0], q_dev.shape[1]
+        check(lib().kvcache_mla_decode_lse_dev(self._h, layer, n, _np_ptr(s), _dptr(q_dev), H, scale, _dptr(out_dev),
+                                               _dptr(lse_dev), _stream(stream)), "mlaDecodeLse_dev")
+
+    def mlaAttentionBatchLse_dev(self, layer, seq, start_pos, q_dev, scale, out_dev, lse_dev, stream=None):
+        """mlaAttentionBatch_dev that also writes lse [n_pos][H]."""
+        n, H = q_dev.shape[0], q_dev.shape[1]
+        check(lib().kvcache_mla_attention_batch_lse_dev(self._h, layer, seq, start_pos, n, _dptr(q_dev), H, scale,
+                                                        _dptr(out_dev), _dptr(lse_dev), _stream(stream)),
+              "mlaAttentionBatchLse_dev")
+
+    def attnMass_dev(self, layer, seq_ids, q_dev, lse_dev, scale, mass_dev, decay=1.0, old_lens=None, stream=None):
+        """mass_dev [n][positions] f32 += the attention weights of q_dev [n][n_q][H][W] (or [n][H][W]), the
+        queries of each sequence's newest n_q positions, with their log-sum-exp lse_dev [n][n_q][H].
+        old_lens (host): sums of positions from there on start anew."""
+        s = np.ascontiguousarray(seq_ids, np.uint32)
+        n, H = q_dev.shape[0], q_dev.shape[-2]
+        n_q = q_dev.shape[1] if q_dev.dim() == 4 else 1
+        old = None if old_lens is None else np.ascontiguousarray(old_lens, np.uint32)
+        if (s.size != n or not (q_dev.is_contiguous() and lse_dev.is_contiguous()) or lse_dev.numel() != n * n_q * H
+                or mass_dev.shape[0] != n or not mass_dev.is_contiguous() or (old is not None and old.size != n)):
+            raise ValueError("attnMass_dev: contiguous q [n][n_q][H][W], lse [n][n_q][H], mass [n][positions]")
+        check(lib().kvcache_attn_mass_dev(self._h, layer, n, _np_ptr(s), n_q, _dptr(q_dev), _dptr(lse_dev), H, scale,
+                                          decay, None if old is None else _np_ptr(old), _dptr(mass_dev),
+                                          mass_dev.shape[1], _stream(stream)), "attnMass_dev")
+
+    def evict_dev(self, seq_ids, budget, mass_dev, n_sink=0, n_recent=0, keep_dev=None, stream=None):
+        """Bring the listed sequences longer than `budget` down to budget rows in every layer by
+        mass_dev [n_layers][n][positions] (moved along); keep_dev [n_layers][n][budget] receives the
+        kept positions.  Their lengths become budget; the blocks behind are freed."""
+        s = np.ascontiguousarray(seq_ids, np.uint32)
+        if (mass_dev.dim() != 3 or mass_dev.shape[:2] != (self.n_layers, s.size) or not mass_dev.is_contiguous() or
+                (keep_dev is not None and (keep_dev.shape != (self.n_layers, s.size, budget) or
+                                           not keep_dev.is_contiguous()))):
+            raise ValueError("evict_dev: contiguous mass [n_layers][n][positions], keep [n_layers][n][budget]")
+        check(lib().kvcache_evict_dev(self._h, s.size, _np_ptr(s), budget, n_sink, n_recent, _dptr(mass_dev),
+                                      mass_dev.stride(0), mass_dev.shape[2], _dptr(keep_dev), _stream(stream)),
+              "evict_dev")
 
     @property
     def last_launches(self):
