@@ -658,8 +658,9 @@ int kvcache_attn_mass_dev(kvcache* c, uint32_t layer, uint32_t n, const uint32_t
  * (KVCU_ERR_OUT_OF_BLOCKS where none is free; nothing is evicted then), and
  * rewritten blocks leave the prefix cache.  keep_dev (device, may be NULL)
  * receives the kept positions [n_layers][n][budget].  Call it between steps,
- * when every layer holds the sequences' rows; it must be ordered after the
- * calls that read them and before those that reuse the blocks (one stream). */
+ * when every layer holds the sequences' rows, ordered after the calls that
+ * wrote or read them; the cache's next append, step, decode or gather, on any
+ * stream, runs after it. */
 int kvcache_evict_dev(kvcache* c, uint32_t n, const uint32_t* seq_ids, uint32_t budget, uint32_t n_sink,
                       uint32_t n_recent, float* mass_dev, uint64_t mass_layer_stride, uint64_t mass_stride,
                       uint32_t* keep_dev, void* stream);

@@ -271,6 +271,13 @@ int stage_acquire(HostStage& h, size_t n) {
   return KVCU_OK;
 }
 
+// An eviction still running on another stream reads the tables and lengths of before
+// and moves rows: `st` continues after it.
+int after_eviction(kvcache* c, cudaStream_t st) {
+  return c->bound_done ? kvcu_check_cuda(cudaStreamWaitEvent(st, c->bound_done, 0), "cudaStreamWaitEvent(eviction)")
+                       : KVCU_OK;
+}
+
 int stage_upload(HostStage& h, uint32_t* dst, size_t n, cudaStream_t st) {
   KVCU_CUDA(cudaMemcpyAsync(dst, h.p, n * 4, cudaMemcpyHostToDevice, st));
   KVCU_CUDA(cudaEventRecord(h.done, st));
@@ -299,6 +306,7 @@ int sync_tables(kvcache* c, cudaStream_t st) {
   const size_t nflat = std::max<size_t>(total, 1);
   int rc = stage_acquire(c->up_toff, nseq + 1);
   if (!rc) rc = stage_acquire(c->up_tables, nflat);
+  if (!rc) rc = after_eviction(c, st);
   if (!rc) rc = ensure_dev(&c->d_toff, &c->d_toff_cap, nseq + 1);
   if (!rc) rc = ensure_dev(&c->d_tables, &c->d_tables_cap, nflat);
   if (rc) return rc;
@@ -327,6 +335,7 @@ int sync_lens(kvcache* c, cudaStream_t st) {
                                              : KVCU_OK;
   const size_t nseq = c->seqs.size();
   int rc = stage_acquire(c->up_lens, std::max<size_t>(nseq, 1));
+  if (!rc) rc = after_eviction(c, st);
   if (!rc) rc = ensure_dev(&c->d_lens, &c->d_lens_cap, nseq);
   if (rc) return rc;
   for (size_t s = 0; s < nseq; ++s) c->up_lens.p[s] = c->seqs[s].len;
@@ -835,8 +844,8 @@ int guarded(const char* what, F f) {
 // call before (on whichever stream) is through with it.
 int bound_acquire(kvcache* c, size_t words, size_t staged, cudaStream_t st) {
   if (!c->bound_done) KVCU_CUDA(cudaEventCreateWithFlags(&c->bound_done, cudaEventDisableTiming));
-  else KVCU_CUDA(cudaStreamWaitEvent(st, c->bound_done, 0));
-  const int rc = ensure_dev(&c->d_bound, &c->d_bound_cap, words);
+  int rc = after_eviction(c, st);
+  if (!rc) rc = ensure_dev(&c->d_bound, &c->d_bound_cap, words);
   return rc ? rc : stage_acquire(c->up_bound, staged);
 }
 
@@ -1470,6 +1479,7 @@ int kvcache_evict_dev(kvcache* c, uint32_t n, const uint32_t* seq_ids, uint32_t 
     if (rc) return rc;
     for (uint32_t b = 0; b < n; ++b)
       if (c->seqs[seq_ids[b]].len > budget) seq_truncate(c, seq_ids[b], budget);
+    if (any) c->tables_dirty = c->lens_dirty = true;  // the next upload, on any stream, waits for the moves
     c->last_launches = 2;
     return KVCU_OK;
   });
