@@ -299,7 +299,7 @@ uint32_t kvcu_decode_last_launches(const kvcu_decode_ws* ws);
 #define KVCU_DECODE_CUDA_CORE 1
 #define KVCU_DECODE_TENSOR_CORE 2
 int kvcu_decode_ws_set_impl(kvcu_decode_ws* ws, int impl);
-/* Every wait of the tensor-core decode kernel is bounded: after `cycles` SM
+/* Every wait of the tensor-core decode and attention-mass kernels is bounded: after `cycles` SM
  * clocks (0 = the default, 2^31, about a second at 1.9 GHz) the CTA records
  * KVCU_STATUS_TIMEOUT in the pool's status word, all its roles unwind, its
  * in-flight copies and MMAs are waited for (with the same bound) and its TMEM
@@ -308,8 +308,8 @@ int kvcu_decode_ws_set_impl(kvcu_decode_ws* ws, int impl);
 int kvcu_decode_ws_set_wait_limit(kvcu_decode_ws* ws, uint64_t cycles);
 /* Test hook for that unwind, needing no GPU fault: in the tensor-core kernel,
  * every CTA's producer skips the copy and the arrival of the first slice of
- * its tile number `tile` (0-based, counted over the CTA's whole range), so the
- * waits on that tile run out.  0xFFFFFFFF turns it off (the default). */
+ * its tile number `tile` (0-based, counted over the CTA's whole range; kvcu_attn_mass:
+ * the first units of a tile of 256 rows), so the waits on that tile run out.  0xFFFFFFFF turns it off (the default). */
 int kvcu_decode_ws_test_withhold(kvcu_decode_ws* ws, uint32_t tile);
 int kvcu_decode_last_impl(const kvcu_decode_ws* ws);
 

@@ -169,6 +169,7 @@ struct TcMass {
   MassArgs m;
   uint32_t box_rows;
   long long wait_limit;
+  uint32_t withhold_plus1;  // test hook: 0, or 1 + the tile of each CTA whose first units are withheld
 };
 
 // Whether the phase is over, for the converged warp: all lanes or none.
@@ -398,6 +399,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                 const uint32_t nth = Q8 ? filled[pr] + u : filled[pr] + u / 2, ring = Q8 ? pr : 2 * pr + (u & 1u);
                 const uint32_t slot = ring * M::DEPTH + nth % M::DEPTH, width = Q8 && u == 4 ? 64u : 128u;
                 if (!(ok = wait(M::B_UE + slot, ((nth / M::DEPTH) & 1u) ^ 1u))) break;
+                if (u == 0 && ti == t.withhold_plus1) continue;  // no copy and no arrival: its readers' waits run out
                 if (lane == 0) kvtc::mbar_arrive_tx(bar(M::B_UF + slot), __popc(of[pr]) * t.box_rows * width);
                 __syncwarp();
                 if (good && pair == pr) {
@@ -735,7 +737,7 @@ int make_maps(const kvcu_pool* p, uint32_t box_rows, CUtensorMap* wide, CUtensor
 }
 
 template <bool Q8, int NC>
-int launch_mass(const kvcu_pool* pool, const MassArgs& a, uint32_t grid, long long wait_limit, cudaStream_t st) {
+int launch_mass(const kvcu_pool* pool, const MassArgs& a, const kvcu_decode_ws* ws, cudaStream_t st) {
   const int rc = kvcu_configure_once(
       reinterpret_cast<const void*>(k_mass<Q8, NC>),
       [](const void*) {
@@ -753,27 +755,27 @@ int launch_mass(const kvcu_pool* pool, const MassArgs& a, uint32_t grid, long lo
       },
       nullptr);
   if (rc) return rc;
-  TcMass t = {a, HALF, wait_limit};
+  TcMass t = {a, HALF, ws->wait_limit ? (long long)ws->wait_limit : (1ll << 31), ws->withhold_plus1};
   while (pool->block_size % t.box_rows) t.box_rows /= 2;  // block sizes are multiples of 16
   CUtensorMap wide, tail;
   const int rm = make_maps(pool, t.box_rows, &wide, &tail);
   if (rm) return rm;
   return kvcu_check_cuda(
-      kvcu_launch_pdl(k_mass<Q8, NC>, dim3(grid), dim3(TC_THREADS), Map<Q8, NC>::ALLOC, st, wide, tail, t),
+      kvcu_launch_pdl(k_mass<Q8, NC>, dim3((uint32_t)ws->decode_ctas), dim3(TC_THREADS), Map<Q8, NC>::ALLOC, st, wide, tail, t),
       "attention mass launch");
 }
 
 // Columns of a chunk: a chunk costs its columns' scaling and exponentials and, whatever
 // their number, the rows' unpacking (as much as about 30 columns).
 template <bool Q8>
-int launch_chunks(const kvcu_pool* pool, const MassArgs& a, uint32_t grid, long long limit, cudaStream_t st) {
+int launch_chunks(const kvcu_pool* pool, const MassArgs& a, const kvcu_decode_ws* ws, cudaStream_t st) {
   const uint32_t cols = a.n_q * a.n_heads;
   auto cost = [&](uint32_t nc) { return (uint64_t)((cols + nc - 1) / nc) * (nc + 30); };
   if (cost(8) <= cost(16) && cost(8) <= cost(20) && cost(8) <= cost(24))
-    return launch_mass<Q8, 8>(pool, a, grid, limit, st);
-  if (cost(16) <= cost(20) && cost(16) <= cost(24)) return launch_mass<Q8, 16>(pool, a, grid, limit, st);
-  if (cost(20) <= cost(24)) return launch_mass<Q8, 20>(pool, a, grid, limit, st);
-  return launch_mass<Q8, 24>(pool, a, grid, limit, st);
+    return launch_mass<Q8, 8>(pool, a, ws, st);
+  if (cost(16) <= cost(20) && cost(16) <= cost(24)) return launch_mass<Q8, 16>(pool, a, ws, st);
+  if (cost(20) <= cost(24)) return launch_mass<Q8, 20>(pool, a, ws, st);
+  return launch_mass<Q8, 24>(pool, a, ws, st);
 }
 
 struct DevScope {
@@ -854,11 +856,9 @@ extern "C" int kvcu_attn_mass(kvcu_decode_ws* ws, kvcu_pool* pool, uint32_t laye
   a.mass = mass;
   a.mass_stride = mass_stride;
   const cudaStream_t st = (cudaStream_t)stream;
-  const uint32_t grid = (uint32_t)ws->decode_ctas;
   if (pool->rows() > 0x7FFFFFFFull) {
     kvcu_set_error("kvcu_attn_mass: %llu rows, TMA coordinates reach 2^31 - 1", (unsigned long long)pool->rows());
     return KVCU_ERR_UNSUPPORTED;
   }
-  const long long limit = ws->wait_limit ? (long long)ws->wait_limit : (1ll << 31);
-  return pool->quantized ? launch_chunks<true>(pool, a, grid, limit, st) : launch_chunks<false>(pool, a, grid, limit, st);
+  return pool->quantized ? launch_chunks<true>(pool, a, ws, st) : launch_chunks<false>(pool, a, ws, st);
 }

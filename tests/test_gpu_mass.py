@@ -314,27 +314,30 @@ def test_refusals(kv):
 
 
 @pytest.mark.parametrize("quant", [True, False])
-def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(kv, quant):
-    """With a limit of a few clocks the first wait that is not over at once gives up: the status says so,
-    nothing hangs, and the same workspace gives the same bits as before."""
+@pytest.mark.parametrize("tile", [0, 1])
+def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(kv, quant, tile):
+    """Units that are never copied: the waits on them end, the status says so, and the same workspace
+    gives the same bits as before."""
     import torch
 
-    cache = Paged(kv, [9000, 3000, 20000, 64], 64, quant, seed=11)
+    cache = Paged(kv, [60000, 3000, 20000, 700], 64, quant, seed=11)  # more than two tiles to a CTA
     q, lse = queries(cache, range(4), 1, 20, 6)
     ws = kv.DecodeWorkspace(0, 4, 20)
     ws.plan(cache.pool, cache.lens_dev)
     new = torch.zeros(4, dtype=torch.int32, device="cuda")
 
     def run():
-        m = torch.zeros(4, 20000, device="cuda")
+        m = torch.zeros(4, 60000, device="cuda")
         ws.attn_mass(cache.pool, 0, q, lse, cache.toff, cache.tables, cache.lens_dev, SCALE, m, old_lens=new)
         torch.cuda.synchronize()
         return m
 
     want = run()
     assert cache.pool.status() == 0
-    ws.set_wait_limit(1)
+    ws.set_wait_limit(1 << 22)  # about 2 ms
+    ws.test_withhold(tile)
     run()
     assert cache.pool.status() & 0x10
+    ws.test_withhold(0xFFFFFFFF)
     ws.set_wait_limit(0)
     assert torch.equal(run(), want) and cache.pool.status() == 0
