@@ -1,0 +1,435 @@
+// kvcu_mass_wide.cu — the attention mass of Q8_0 rows for many columns (queries x heads).
+//
+// k_mass (kvcu_mass.cu) adds a row's 18 block sums in f32, exact int8 values times q:
+// the best for a step's few columns, but its scaling grows with the columns and its
+// chunks re-unpack the rows.  Here a row's value, int8 times its block's scale (19 bits),
+// is the exact sum of two f16 parts, so one accumulator serves all of K = 576: a GEMM
+//   S[row][column] = A_hi B_hi + A_lo B_hi + A_hi B_lo       (low times low < 2^-22)
+// with 128 rows to a tile (A, unpacked into TMEM), up to 192 columns to a chunk (B, q's
+// parts made by k_mass_wide_q) and the exponentials as its epilogue.
+//   A row's scales are brought to at most 2^8 by a power of two of the row; its parts
+// are exact for blocks with scales down to 2^-21 of the row's largest, and within
+// 2^-39 of the row's largest value below that.  The tensor cores' own f32 accumulation
+// drops bits of each addend, so a unit's sum is taken out of TMEM after every third of
+// K and added in registers: 36 additions of the tensor core to a sum.
+//
+// A unit is (tile, chunk), 9 stages of 64 elements each.  Per stage of N columns the
+// MMAs take 12 x N/2 clocks; B is streamed from L2, 256 N bytes to a stage (43 B a clock
+// of the 71 an SM can take), as a chunk of all of K would not fit beside its ring.
+//   warps 0-15   each thread has one row of the tile and in every second stage one of its
+//                two blocks: two loads, 32 values to f16 parts, into the stage's TMEM
+//                buffer; it drains a quarter of the columns of its row
+//   warp 16      producer: TMA boxes of 64 elements x N columns of one part
+//   warp 17      issues the MMAs
+#include "kvcu_mass.cuh"
+
+using namespace kvmass;
+
+namespace {
+
+constexpr int COMPUTE = 16, PRODUCER = 16, ISSUER = 17, THREADS = (COMPUTE + 4) * 32;
+// Registers: launched with 96 a thread; the last warpgroup gives to the four others.
+constexpr int LAUNCH_REGS = 96, SERVICE_REGS = 64, COMPUTE_REGS = 104;
+static_assert(COMPUTE * COMPUTE_REGS + 4 * SERVICE_REGS <= (COMPUTE + 4) * LAUNCH_REGS,
+              "register split exceeds the launch allocation");
+constexpr uint32_t ROWS = 128, STAGES = W / 64;
+constexpr uint32_t MAX_N = 192, MAX_BLOCKS = MAX_N / 32;  // columns of a chunk; blocks of 8 a thread drains
+constexpr uint32_t GROUP = 3;                             // stages to a drain
+constexpr uint32_t RING_BYTES = 8 * MAX_N * 128, MAX_SLOTS = 16;
+constexpr uint32_t TM_A = 2 * MAX_N, TM_COLS = 512;  // TMEM: two D regions, then two buffers of 64 columns
+constexpr uint32_t SUMS = RING_BYTES;                // [2][3][ROWS]
+// barriers
+constexpr int B_BF = 0, B_BE = MAX_SLOTS, B_AF = 2 * MAX_SLOTS, B_AE = B_AF + 2, B_DF = B_AE + 2, B_DE = B_DF + 2,
+              B_SF = B_DE + 2, B_SE = B_SF + 2, B_FINAL = B_SE + 2, NUM_BARS = B_FINAL + 1;
+constexpr uint32_t BARS = SUMS + 2 * 3 * ROWS * 4, MISC = BARS + NUM_BARS * 8, ALLOC = MISC + 16 + 1024;
+static_assert(ALLOC <= 232448 && TM_A + 2 * 64 <= TM_COLS, "budgets");
+constexpr long long DRAIN_LIMIT = 1ll << 31;
+
+struct Wide {
+  MassArgs m;
+  uint32_t q0, cols, chunks, width, padded;  // of an entry: first query, columns, chunks of `width`, chunks * width
+  uint32_t slots;                            // of the ring
+  const float4* col;                         // [n][padded]: scale, -lse, limit (bits)
+  long long wait_limit;
+  uint32_t withhold_plus1;  // test hook: 0, or 1 + the tile of each CTA whose first unit of B is withheld
+};
+
+void shape(uint32_t cols, uint32_t* chunks, uint32_t* width) {
+  *chunks = (cols + MAX_N - 1) / MAX_N;
+  *width = ((cols + *chunks - 1) / *chunks + 31) / 32 * 32;
+}
+
+// The columns' parts, [n][hi, lo][padded][W] f16, and constants; a warp to a column.
+__global__ void __launch_bounds__(256) k_mass_wide_q(const Wide t, __half* parts, float4* consts) {
+  kvcu_pdl_wait();
+  const MassArgs& a = t.m;
+  const uint64_t id = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const uint32_t lane = threadIdx.x & 31u;
+  if (id >= (uint64_t)a.n * t.padded) return;
+  const uint32_t b = (uint32_t)(id / t.padded), c = (uint32_t)(id % t.padded);
+  const bool live = c < t.cols;
+  const uint32_t i = t.q0 + c / a.n_heads;
+  const uint64_t column = ((uint64_t)b * a.n_q + i) * a.n_heads + c % a.n_heads;
+  const float4* src = reinterpret_cast<const float4*>(a.q + column * W);
+  float4 x[5];
+  float amax = 0.f;
+#pragma unroll
+  for (int k = 0; k < 5; ++k) {
+    const uint32_t f = lane + 32 * k;
+    x[k] = live && f < W / 4 ? src[f] : make_float4(0.f, 0.f, 0.f, 0.f);
+    amax = fmaxf(fmaxf(fmaxf(amax, fabsf(x[k].x)), fmaxf(fabsf(x[k].y), fabsf(x[k].z))), fabsf(x[k].w));
+  }
+  const uint32_t field = scale_field(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
+  const float up = __uint_as_float(field << 23);
+  uint2* hi = reinterpret_cast<uint2*>(parts + ((uint64_t)b * 2 * t.padded + c) * W);
+  uint2* lo = hi + (uint64_t)t.padded * (W / 4);
+#pragma unroll
+  for (int k = 0; k < 5; ++k) {
+    const uint32_t f = lane + 32 * k;
+    if (f >= W / 4) continue;
+    uint2 h, l;
+    split(x[k].x * up, x[k].y * up, &h.x, &l.x);
+    split(x[k].z * up, x[k].w * up, &h.y, &l.y);
+    hi[f] = h;
+    lo[f] = l;
+  }
+  if (lane == 0) {
+    constexpr double LOG2E = 1.4426950408889634;
+    const float l = live ? a.lse[column] : -INFINITY;
+    const uint32_t behind = live ? a.n_q - 1 - i : 0u, len = entry_of(a, b, false).len;
+    // a column past the last, or a query that saw nothing, has no positions
+    const uint32_t limit = l == -INFINITY || len <= behind ? 0u : len - behind;
+    consts[(uint64_t)b * t.padded + c] = make_float4((float)(a.scale * LOG2E) * __uint_as_float((254u - field) << 23),
+                                                     (float)(-l * LOG2E), __uint_as_float(limit), 0.f);
+  }
+}
+
+__global__ void __launch_bounds__(THREADS, 1) k_mass_wide(const __grid_constant__ CUtensorMap map, const Wide t) {
+  const MassArgs& a = t.m;
+  extern __shared__ char raw[];
+  char* sm = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t base = kvtc::smem_u32(sm);
+  const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(sm + MISC + 4);
+  auto bar = [&](uint32_t i) { return base + BARS + 8u * i; };
+  auto wait = [&](uint32_t i, uint32_t parity) { return wait_bar(bar(i), parity, abort_flag, t.wait_limit); };
+  if (tid == 0) {
+    auto init = [&](int first, int n, uint32_t count) {
+      for (int i = 0; i < n; ++i) kvtc::mbar_init(bar(first + i), count);
+    };
+    init(B_BF, MAX_SLOTS, 1);
+    init(B_BE, MAX_SLOTS, 1);
+    init(B_AF, 2, 8);
+    init(B_AE, 2, 1);
+    init(B_DF, 2, 1);
+    init(B_DE, 2, COMPUTE);
+    init(B_SF, 2, 12);
+    init(B_SE, 2, 4);
+    init(B_FINAL, 1, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == ISSUER) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + MISC), "r"(TM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  kvcu_pdl_wait();
+  kvtc::tc_fence_before();
+  __syncthreads();
+  kvtc::tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sm + MISC);
+  const uint32_t n_items = a.meta[0], n_ranges = a.meta[1];
+  const uint32_t it0 = blockIdx.x < n_ranges ? min(a.ranges[blockIdx.x], n_items) : n_items;
+  const uint32_t it1 = blockIdx.x < n_ranges ? min(a.ranges[blockIdx.x + 1], n_items) : n_items;
+  const uint32_t unit_bytes = t.width * 128u;
+  bool ok = true;
+
+  if (warp >= COMPUTE) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SERVICE_REGS));
+  if (warp == PRODUCER) {
+    // ---------------------------------------------------------------- producer
+    if (blockIdx.x == 0 && lane == 0 && n_ranges > gridDim.x) atomicOr(a.status, KVCU_STATUS_BAD_PLAN);
+    uint32_t slot = 0, lap = 0, tile = 0;
+    uint32_t sent = 0;  // lane k: units sent through slot k
+    for (uint32_t it = it0; ok && it < it1; ++it) {
+      const kvcu_item w = a.items[it];
+      const uint32_t end = min(w.end, entry_of(a, w.b, lane == 0).len);
+      for (uint32_t p0 = w.start; ok && p0 < end; p0 += ROWS) {
+        ++tile;
+        for (uint32_t ch = 0; ok && ch < t.chunks; ++ch)
+          for (uint32_t u = 0; u < 2 * STAGES; ++u) {  // stage u / 2, part u % 2
+            if (!(ok = wait(B_BE + slot, (lap & 1u) ^ 1u))) break;
+            // test hook: no copy and no arrival, the waits on it run out
+            if (!(u == 0 && ch == 0 && tile == t.withhold_plus1)) {
+              if (lane == 0) {
+                kvtc::mbar_arrive_tx(bar(B_BF + slot), unit_bytes);
+                tma_2d(base + slot * unit_bytes, &map, (int)(u / 2 * 64),
+                       (int)((w.b * 2 + (u & 1u)) * t.padded + ch * t.width), bar(B_BF + slot));
+              }
+              __syncwarp();
+              sent += lane == slot;
+            }
+            if (++slot == t.slots) slot = 0, ++lap;
+          }
+      }
+    }
+    if (!ok) {  // the copies in flight must land before the CTA leaves
+      const long long t0 = clock64();
+      while (sent && !kvtc::mbar_try(bar(B_BF + lane), (sent - 1) & 1u) && clock64() - t0 <= DRAIN_LIMIT) {
+      }
+      __syncwarp();
+    }
+  } else if (warp == ISSUER) {
+    // ---------------------------------------------------------------- MMA issuer
+    // kind::f16: D f32 (bit 4), A and B f16, both K-major, N >> 3 at bit 17, M >> 4 at bit 24
+    const uint32_t idesc = (1u << 4) | ((t.width >> 3) << 17) | ((ROWS >> 4) << 24);
+    uint32_t x = 0, g = 0, slot = 0, lap = 0;  // stages, groups, and the ring's place
+    for (uint32_t it = it0; ok && it < it1; ++it) {
+      const kvcu_item w = a.items[it];
+      const uint32_t end = min(w.end, entry_of(a, w.b, false).len);
+      const uint32_t units = w.start < end ? (end - w.start + ROWS - 1) / ROWS * t.chunks : 0u;
+      for (uint32_t s = 0; ok && s < units * STAGES; ++s, ++x) {
+        const bool first = s % GROUP == 0;
+        if (first && !(ok = wait(B_DE + (g & 1u), ((g >> 1) & 1u) ^ 1u))) break;
+        if (!(ok = wait(B_AF + (x & 1u), (x >> 1) & 1u))) break;
+        const uint32_t td = tmem + (g & 1u) * MAX_N, ta = tmem + TM_A + (x & 1u) * 64u;
+        for (uint32_t part = 0; part < 2; ++part) {
+          if (!(ok = wait(B_BF + slot, lap & 1u))) break;
+          kvtc::tc_fence_after();
+          if (kvtc::elect_one()) {
+            const uint64_t at = kvtc::smem_desc(base + slot * unit_bytes, 16, 1024, kvtc::LAYOUT_SW128);
+#pragma unroll
+            for (uint32_t ks = 0; ks < 4; ++ks) {
+              mma_ts(td, ta + ks * 8u, at + ks * 2u, idesc, first && part == 0 && ks == 0 ? 0u : 1u);
+              if (part == 0) mma_ts(td, ta + 32u + ks * 8u, at + ks * 2u, idesc, 1u);
+            }
+            kvtc::mma_commit(bar(B_BE + slot));
+            if (part) {
+              kvtc::mma_commit(bar(B_AE + (x & 1u)));
+              if (s % GROUP == GROUP - 1) kvtc::mma_commit(bar(B_DF + (g & 1u)));
+            }
+          }
+          __syncwarp();
+          if (++slot == t.slots) slot = 0, ++lap;
+        }
+        if (!ok) break;
+        g += s % GROUP == GROUP - 1;
+      }
+    }
+    // all issued MMAs retire before TMEM is freed
+    if (kvtc::elect_one()) kvtc::mma_commit(bar(B_FINAL));
+    __syncwarp();
+    const long long t0 = clock64();
+    while (!kvtc::mbar_try(bar(B_FINAL), 0) && clock64() - t0 <= DRAIN_LIMIT) {
+    }
+  } else if (warp < COMPUTE) {
+    // ---------------------------------------------------------------- rows and sums
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(COMPUTE_REGS));
+    const uint32_t wg = warp >> 2, pair = wg >> 1, half = wg & 1u, r = (warp & 3u) * 32u + lane;
+    const uint32_t lanes = (warp & 3u) * 32u << 16, quarter = t.width / 4, blocks = t.width / 32;
+    const uint32_t ta = tmem + lanes + TM_A + pair * 64u + half * 16u;
+    float* sums = reinterpret_cast<float*>(sm + SUMS) + r;
+    uint32_t x = 0, drained = 0, tiles = 0;  // stages begun by all, groups drained, tiles finished
+    float tot[MAX_BLOCKS][8], run = 0.f;
+    // the unit that the next group to drain belongs to
+    struct Unit {
+      uint32_t b, p, old, c0, flags;  // flags: 1 the row is there, 2 the tile's last chunk
+      float down;                     // the row's power of two, taken back
+    } cur = {}, prev = {};
+    uint32_t cur_first = 0;  // groups before the current unit's
+
+    auto finish = [&](const Unit& u) -> bool {  // the unit's weights; after the last chunk the tile's masses
+      const float4* col = t.col + (uint64_t)u.b * t.padded + u.c0 + wg * quarter;
+#pragma unroll
+      for (uint32_t i = 0; i < MAX_BLOCKS; ++i) {
+        if (i >= blocks) continue;
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) {
+          const float4 c = __ldg(col + i * 8 + k);
+          const float w = exp2_approx(fmaf(tot[i][k], c.x * u.down, c.y));
+          run += u.p < __float_as_uint(c.z) ? w : 0.f;
+        }
+      }
+      if (!(u.flags & 2u)) return true;
+      const uint32_t f = tiles & 1u, parity = (tiles >> 1) & 1u;
+      if (wg) {
+        if (!wait(B_SE + f, parity ^ 1u)) return false;
+        sums[(f * 3 + wg - 1) * ROWS] = run;
+        __syncwarp();
+        if (lane == 0) kvtc::mbar_arrive(bar(B_SF + f));
+      } else {
+        float* out = a.mass + (uint64_t)u.b * a.mass_stride + u.p;
+        const float before = (u.flags & 1u) && (t.q0 || u.p < u.old) ? *out : 0.f;
+        if (!wait(B_SF + f, parity)) return false;
+#pragma unroll
+        for (int k = 0; k < 3; ++k) run += sums[(f * 3 + k) * ROWS];
+        __syncwarp();
+        if (lane == 0) kvtc::mbar_arrive(bar(B_SE + f));
+        if (u.flags & 1u) *out = fmaf(t.q0 ? 1.f : a.decay, before, run);
+      }
+      run = 0.f;
+      ++tiles;
+      return true;
+    };
+    // the sums of the oldest group that was not taken yet
+    auto drain = [&]() -> bool {
+      const uint32_t f = drained & 1u, part = drained % (STAGES / GROUP);
+      if (!wait(B_DF + f, (drained >> 1) & 1u)) return false;
+      kvtc::tc_fence_after();
+      const uint32_t td = tmem + lanes + f * MAX_N + wg * quarter;
+#pragma unroll
+      for (uint32_t i = 0; i < MAX_BLOCKS; ++i) {
+        if (i >= blocks) continue;
+        uint32_t v[8];
+        kvtc::tmem_ld<8>(td + i * 8, v);
+        kvtc::tmem_wait_ld();
+        kvtc::reg_fence(v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) tot[i][k] = part ? tot[i][k] + __uint_as_float(v[k]) : __uint_as_float(v[k]);
+      }
+      kvtc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) kvtc::mbar_arrive(bar(B_DE + f));
+      const bool of_prev = drained < cur_first;
+      ++drained;
+      return part != STAGES / GROUP - 1 || finish(of_prev ? prev : cur);
+    };
+
+    for (uint32_t it = it0; ok && it < it1; ++it) {
+      const kvcu_item w = a.items[it];
+      const Entry e = entry_of(a, w.b, false);
+      const uint32_t end = min(w.end, e.len);
+      for (uint32_t p0 = w.start; ok && p0 < end; p0 += ROWS) {
+        const uint32_t p = p0 + r, blk = p < end ? a.tables[e.t0 + p / a.block_size] : 0xFFFFFFFFu;
+        const bool good = blk < a.num_blocks;
+        if (p < end && !good) atomicOr(a.status, KVCU_STATUS_BAD_BLOCK);
+        const uint64_t row = good ? ((uint64_t)a.layer * a.num_blocks + blk) * a.block_size + p % a.block_size : 0;
+        const uint4* values = reinterpret_cast<const uint4*>(a.qs + row * W + half * 32u);
+        const uint32_t* scales = reinterpret_cast<const uint32_t*>(a.sc + row * NBLK);  // rows are 36 bytes
+        // the power of two that brings the largest scale to [2^7, 2^8)
+        uint32_t top = 0;
+#pragma unroll
+        for (uint32_t s = 0; s < STAGES; ++s) {
+          const uint32_t two = good ? __ldg(scales + s) & 0x7fff7fffu : 0u;
+          top = max(top, max(two & 0xffffu, two >> 16));
+        }
+        const uint32_t tf = __float_as_uint(__half2float(__ushort_as_half((unsigned short)top)));
+        const uint32_t field = top == 0u || top >= 0x7c00u ? 127u : 261u - (tf >> 23);  // 2^(7 - exponent)
+        const float up = __uint_as_float(field << 23), down = __uint_as_float((254u - field) << 23);
+        uint32_t s = (x ^ pair) & 1u;  // this pair's first stage
+        uint4 d0 = {}, d1 = {};
+        uint32_t sc = 0;
+        auto load = [&](uint32_t at) {
+          if (!good) return;
+          d0 = __ldg(values + at * 4);
+          d1 = __ldg(values + at * 4 + 1);
+          sc = __ldg(scales + at);
+        };
+        load(s);
+        for (uint32_t ch = 0; ok && ch < t.chunks; ++ch) {
+          prev = cur;
+          cur = {w.b, p, t.q0 ? e.len : e.old, ch * t.width, (good ? 1u : 0u) | (ch + 1 == t.chunks ? 2u : 0u), down};
+          cur_first = x / GROUP;
+          for (s = (x ^ pair) & 1u; s < STAGES; s += 2) {
+            const uint32_t at = x + s;  // of all stages; this pair's buffer's (at >> 1)-th
+            if (!(ok = wait(B_AE + pair, ((at >> 1) & 1u) ^ 1u))) break;
+            const __half one = __float2half_rn(__half2float(__ushort_as_half((unsigned short)(half ? sc >> 16 : sc & 0xffffu))) * up);
+            const __half2 scale = __half2half2(one);
+            auto part = [&](uint4 v, uint32_t to) {  // 16 values: eight columns of each part
+              uint32_t h[8], hi[8], lo[8];
+              int8_to_f16(v.x, h);
+              int8_to_f16(v.y, h + 2);
+              int8_to_f16(v.z, h + 4);
+              int8_to_f16(v.w, h + 6);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const __half2 y = *reinterpret_cast<const __half2*>(&h[k]), top = __hmul2_rn(y, scale);
+                const __half2 rest = __hfma2(y, scale, __hneg2(top));
+                hi[k] = *reinterpret_cast<const uint32_t*>(&top);
+                lo[k] = *reinterpret_cast<const uint32_t*>(&rest);
+              }
+              kvtc::tmem_st<8>(to, hi);
+              kvtc::tmem_st<8>(to + 32, lo);
+            };
+            part(d0, ta);
+            part(d1, ta + 8);
+            load(s + 2 < STAGES ? s + 2 : (s + 2) - STAGES);  // the next one of this tile, if there is one
+            kvtc::tmem_wait_st();
+            kvtc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) kvtc::mbar_arrive(bar(B_AF + pair));
+            // groups whose MMAs are over: those up to the stage whose buffer was free just now
+            while (ok && GROUP * (drained + 1) + 1 <= at) ok = drain();
+            if (!ok) break;
+          }
+          x += STAGES;
+        }
+      }
+    }
+    while (ok && GROUP * (drained + 1) <= x) ok = drain();
+  }
+  // ---- teardown
+  kvcu_pdl_trigger();
+  __syncwarp();
+  kvtc::tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && *abort_flag) atomicOr(a.status, KVCU_STATUS_TIMEOUT);
+  if (warp == ISSUER) {
+    kvtc::tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TM_COLS) : "memory");
+  }
+}
+
+}  // namespace
+
+namespace kvmass {
+
+uint64_t wide_scratch(uint32_t n, uint32_t cols) {
+  uint32_t chunks, width;
+  shape(cols, &chunks, &width);
+  return (uint64_t)n * chunks * width * (2 * W * sizeof(__half) + sizeof(float4));
+}
+
+int launch_wide(const kvcu_pool* pool, const MassArgs& a, uint32_t q0, uint32_t count, void* scratch,
+                const kvcu_decode_ws* ws, cudaStream_t st) {
+  Wide t = {};
+  t.m = a;
+  t.q0 = q0;
+  t.cols = count * a.n_heads;
+  shape(t.cols, &t.chunks, &t.width);
+  t.padded = t.chunks * t.width;
+  t.slots = RING_BYTES / (t.width * 128u);
+  if (t.slots > MAX_SLOTS) t.slots = MAX_SLOTS;
+  const uint64_t columns = (uint64_t)a.n * t.padded;
+  __half* parts = static_cast<__half*>(scratch);
+  float4* consts = reinterpret_cast<float4*>(parts + columns * 2 * W);
+  t.col = consts;
+  t.wait_limit = ws->wait_limit ? (long long)ws->wait_limit : (1ll << 31);
+  t.withhold_plus1 = ws->withhold_plus1;
+  int rc = kvcu_configure_once(
+      reinterpret_cast<const void*>(k_mass_wide),
+      [](const void*) {
+        // the register split assumes exactly this many at launch: with fewer, setmaxnreg.inc would wait for ever
+        cudaFuncAttributes fa;
+        KVCU_CUDA(cudaFuncGetAttributes(&fa, k_mass_wide));
+        if (fa.numRegs != LAUNCH_REGS) {
+          kvcu_set_error("attn_mass: built with %d registers per thread, the register split needs %d", fa.numRegs,
+                         LAUNCH_REGS);
+          return (int)KVCU_ERR_UNSUPPORTED;
+        }
+        return kvcu_check_cuda(cudaFuncSetAttribute(k_mass_wide, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ALLOC),
+                               "cudaFuncSetAttribute(mass)");
+      },
+      nullptr);
+  if (rc) return rc;
+  CUtensorMap map;
+  rc = make_map(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, parts, 2 * columns, W, 64, t.width);
+  if (rc) return rc;
+  rc = kvcu_check_cuda(kvcu_launch_pdl(k_mass_wide_q, dim3((uint32_t)((columns + 7) / 8)), dim3(256), 0, st, t, parts, consts),
+                       "attention mass columns launch");
+  if (rc) return rc;
+  return kvcu_check_cuda(kvcu_launch_pdl(k_mass_wide, dim3((uint32_t)ws->decode_ctas), dim3(THREADS), ALLOC, st, map, t),
+                         "attention mass launch");
+}
+
+}  // namespace kvmass

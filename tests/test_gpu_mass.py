@@ -313,6 +313,87 @@ def test_refusals(kv):
         ws.attn_mass(cache.pool, 0, q, lse, *args, mass)
 
 
+@pytest.mark.parametrize("n_q,heads,bs", [(8, 8, 64), (3, 32, 16), (20, 10, 48), (48, 32, 128), (5, 20, 256)])
+def test_many_columns(kv, n_q, heads, bs):
+    """Windows of 64 and more columns, from one chunk to eight; 48 x 32 columns of eight entries take
+    several passes over the queries.  Sums of old positions decay once."""
+    import torch
+
+    lens = [n_q, 127, 128, 129, 255, 1, 2500, 640]
+    cache = Paged(kv, lens, bs, True, layers=2, seed=n_q)
+    n = len(lens)
+    q, lse = queries(cache, range(n), n_q, heads, 3, layer=1)
+    mass = torch.rand(n, max(lens) + 3, device="cuda")
+    before = mass.clone()
+    old = [max(0, x - n_q) for x in lens]
+    want, tol = want_mass(cache, range(n), q, lse, mass, 0.9, old, layer=1)
+    ws = kv.DecodeWorkspace(0, n, heads)
+    ws.plan(cache.pool, cache.lens_dev)
+    ws.attn_mass(cache.pool, 1, q, lse, cache.toff, cache.tables, cache.lens_dev, SCALE, mass, decay=0.9,
+                 old_lens=torch.tensor(old, dtype=torch.int32, device="cuda"))
+    assert cache.pool.status() == 0
+    check(mass, want, tol)
+    for b, length in enumerate(lens):
+        assert torch.equal(mass[b, length:], before[b, length:])
+
+
+def test_many_columns_with_uneven_scales(kv):
+    """Blocks of a row whose scales span the f16 range, zeros among them, and a bad block."""
+    import torch
+
+    from pooldata import arrays
+
+    cache = Paged(kv, [300, 900], 32, True, seed=12)
+    _, sc = arrays(cache.pool)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    power = torch.randint(-12, 1, sc.shape, generator=g, device="cuda").float()
+    sc.copy_((sc.float() * 2.0 ** power).half())
+    sc[::5, 3] = 0
+    sc[7::31] = 0
+    n_q, heads = 6, 20
+    q, lse = queries(cache, range(2), n_q, heads, 5)
+    mass = torch.rand(2, 900, device="cuda")
+    before = mass.clone()
+    want, tol = want_mass(cache, range(2), q, lse, mass, 1.0, cache.lens)
+    tables = cache.tables.clone()
+    tables[2] = -1  # positions 64..95 of the first sequence
+    ws = kv.DecodeWorkspace(0, 2, heads)
+    ws.plan(cache.pool, cache.lens_dev)
+    ws.attn_mass(cache.pool, 0, q, lse, cache.toff, tables, cache.lens_dev, SCALE, mass)
+    assert cache.pool.status() == 0x2
+    assert torch.equal(mass[0, 64:96], before[0, 64:96])
+    mass[0, 64:96] = want[0, 64:96].float()
+    check(mass, want, tol)
+
+
+def test_many_columns_withheld_and_again(kv):
+    import torch
+
+    cache = Paged(kv, [30000, 10000], 64, True, seed=13)
+    n_q, heads = 4, 20
+    q, lse = queries(cache, range(2), n_q, heads, 5)
+    ws = kv.DecodeWorkspace(0, 2, heads)
+    ws.plan(cache.pool, cache.lens_dev)
+    new = torch.zeros(2, dtype=torch.int32, device="cuda")
+
+    def run():
+        m = torch.zeros(2, 30000, device="cuda")
+        ws.attn_mass(cache.pool, 0, q, lse, cache.toff, cache.tables, cache.lens_dev, SCALE, m, old_lens=new)
+        torch.cuda.synchronize()
+        return m
+
+    want = run()
+    assert cache.pool.status() == 0
+    ws.set_wait_limit(1 << 22)
+    for tile in (0, 1):
+        ws.test_withhold(tile)
+        run()
+        assert cache.pool.status() & 0x10
+    ws.test_withhold(0xFFFFFFFF)
+    ws.set_wait_limit(0)
+    assert torch.equal(run(), want) and cache.pool.status() == 0
+
+
 @pytest.mark.parametrize("quant", [True, False])
 @pytest.mark.parametrize("tile", [0, 1])
 def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(kv, quant, tile):
