@@ -114,11 +114,6 @@ struct TcMass {
   uint32_t withhold_plus1;  // test hook: 0, or 1 + the tile of each CTA whose first units are withheld
 };
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
-}
 // The q parts of (entry b, columns from c0) and each column's scale, -lse and limit,
 // rows dealt to the compute warps.
 template <bool Q8, int NC>

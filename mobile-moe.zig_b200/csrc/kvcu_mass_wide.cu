@@ -16,9 +16,10 @@
 // A unit is (tile, chunk), 9 stages of 64 elements each.  Per stage of N columns the
 // MMAs take 12 x N/2 clocks; B is streamed from L2, 256 N bytes to a stage (43 B a clock
 // of the 71 an SM can take), as a chunk of all of K would not fit beside its ring.
-//   warps 0-15   each thread has one row of the tile and in every second stage one of its
-//                two blocks: two loads, 32 values to f16 parts, into the stage's TMEM
-//                buffer; it drains a quarter of the columns of its row
+//   warps 0-7    drain: each thread the sums of one row and half of the columns, their
+//                exponentials, and the row's mass
+//   warps 8-15   unpack: each thread one row's 64 values of every second stage, to f16
+//                parts in the stage's TMEM buffer
 //   warp 16      producer: TMA boxes of 64 elements x N columns of one part
 //   warp 17      issues the MMAs
 #include "kvcu_mass.cuh"
@@ -27,21 +28,22 @@ using namespace kvmass;
 
 namespace {
 
-constexpr int COMPUTE = 16, PRODUCER = 16, ISSUER = 17, THREADS = (COMPUTE + 4) * 32;
-// Registers: launched with 96 a thread; the last warpgroup gives to the four others.
-constexpr int LAUNCH_REGS = 96, SERVICE_REGS = 64, COMPUTE_REGS = 104;
-static_assert(COMPUTE * COMPUTE_REGS + 4 * SERVICE_REGS <= (COMPUTE + 4) * LAUNCH_REGS,
+constexpr int DRAIN = 8, UNPACK = 16, PRODUCER = 16, ISSUER = 17, THREADS = 20 * 32;  // warps up to DRAIN, UNPACK
+// Registers: launched with 96 a thread; the drain's sums take what the others leave.
+constexpr int LAUNCH_REGS = 96, DRAIN_REGS = 136, UNPACK_REGS = 72, SERVICE_REGS = 64;
+static_assert(8 * DRAIN_REGS + 8 * UNPACK_REGS + 4 * SERVICE_REGS <= 20 * LAUNCH_REGS,
               "register split exceeds the launch allocation");
 constexpr uint32_t ROWS = 128, STAGES = W / 64;
-constexpr uint32_t MAX_N = 192, MAX_BLOCKS = MAX_N / 32;  // columns of a chunk; blocks of 8 a thread drains
+constexpr uint32_t MAX_N = 192, MAX_BLOCKS = MAX_N / 32;  // columns of a chunk; blocks of 16 a thread drains
 constexpr uint32_t GROUP = 3;                             // stages to a drain
 constexpr uint32_t RING_BYTES = 8 * MAX_N * 128, MAX_SLOTS = 16;
 constexpr uint32_t TM_A = 2 * MAX_N, TM_COLS = 512;  // TMEM: two D regions, then two buffers of 64 columns
-constexpr uint32_t SUMS = RING_BYTES;                // [2][3][ROWS]
+constexpr uint32_t COL = RING_BYTES;  // [2][MAX_N] a chunk's constants
+constexpr uint32_t SUMS = COL + 2 * MAX_N * 16;                // [2][ROWS]
 // barriers
 constexpr int B_BF = 0, B_BE = MAX_SLOTS, B_AF = 2 * MAX_SLOTS, B_AE = B_AF + 2, B_DF = B_AE + 2, B_DE = B_DF + 2,
-              B_SF = B_DE + 2, B_SE = B_SF + 2, B_FINAL = B_SE + 2, NUM_BARS = B_FINAL + 1;
-constexpr uint32_t BARS = SUMS + 2 * 3 * ROWS * 4, MISC = BARS + NUM_BARS * 8, ALLOC = MISC + 16 + 1024;
+              B_SF = B_DE + 2, B_SE = B_SF + 2, B_CF = B_SE + 2, B_CE = B_CF + 2, B_FINAL = B_CE + 2, NUM_BARS = B_FINAL + 1;
+constexpr uint32_t BARS = SUMS + 2 * ROWS * 4, MISC = BARS + NUM_BARS * 8, ALLOC = MISC + 16 + 1024;
 static_assert(ALLOC <= 232448 && TM_A + 2 * 64 <= TM_COLS, "budgets");
 constexpr long long DRAIN_LIMIT = 1ll << 31;
 
@@ -57,6 +59,29 @@ struct Wide {
 void shape(uint32_t cols, uint32_t* chunks, uint32_t* width) {
   *chunks = (cols + MAX_N - 1) / MAX_N;
   *width = ((cols + *chunks - 1) / *chunks + 31) / 32 * 32;
+}
+
+constexpr uint64_t NO_ROW = ~0ull;
+// The row of the pool that position p of the entry has, NO_ROW behind `end` or in a bad block.
+__device__ __forceinline__ uint64_t row_of(const MassArgs& a, const Entry& e, uint32_t p, uint32_t end, bool report) {
+  if (p >= end) return NO_ROW;
+  const uint32_t blk = a.tables[e.t0 + p / a.block_size];
+  if (blk < a.num_blocks) return ((uint64_t)a.layer * a.num_blocks + blk) * a.block_size + p % a.block_size;
+  if (report) atomicOr(a.status, KVCU_STATUS_BAD_BLOCK);
+  return NO_ROW;
+}
+// The exponent field of the power of two that brings the row's largest scale to [2^7, 2^8).
+__device__ __forceinline__ uint32_t scale_of(const MassArgs& a, uint64_t row) {
+  if (row == NO_ROW) return 127u;
+  const uint32_t* scales = reinterpret_cast<const uint32_t*>(a.sc + row * NBLK);
+  uint32_t top = 0;
+#pragma unroll
+  for (uint32_t s = 0; s < STAGES; ++s) {
+    const uint32_t two = __ldg(scales + s) & 0x7fff7fffu;
+    top = max(top, max(two & 0xffffu, two >> 16));
+  }
+  const uint32_t bits = __float_as_uint(__half2float(__ushort_as_half((unsigned short)top)));
+  return top == 0u || top >= 0x7c00u ? 127u : 261u - (bits >> 23);  // 7 - exponent, biased
 }
 
 // The columns' parts, [n][hi, lo][padded][W] f16, and constants; a warp to a column.
@@ -119,12 +144,14 @@ __global__ void __launch_bounds__(THREADS, 1) k_mass_wide(const __grid_constant_
     };
     init(B_BF, MAX_SLOTS, 1);
     init(B_BE, MAX_SLOTS, 1);
-    init(B_AF, 2, 8);
+    init(B_AF, 2, 4);
     init(B_AE, 2, 1);
     init(B_DF, 2, 1);
-    init(B_DE, 2, COMPUTE);
-    init(B_SF, 2, 12);
+    init(B_DE, 2, DRAIN);
+    init(B_SF, 2, 4);
     init(B_SE, 2, 4);
+    init(B_CF, 2, 1);
+    init(B_CE, 2, DRAIN);
     init(B_FINAL, 1, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -145,18 +172,26 @@ __global__ void __launch_bounds__(THREADS, 1) k_mass_wide(const __grid_constant_
   const uint32_t unit_bytes = t.width * 128u;
   bool ok = true;
 
-  if (warp >= COMPUTE) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SERVICE_REGS));
+  if (warp >= UNPACK) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SERVICE_REGS));
   if (warp == PRODUCER) {
     // ---------------------------------------------------------------- producer
     if (blockIdx.x == 0 && lane == 0 && n_ranges > gridDim.x) atomicOr(a.status, KVCU_STATUS_BAD_PLAN);
-    uint32_t slot = 0, lap = 0, tile = 0;
-    uint32_t sent = 0;  // lane k: units sent through slot k
+    uint32_t slot = 0, lap = 0, tile = 0, unit = 0;
+    uint32_t sent = 0;  // lane k: units of B sent through slot k
     for (uint32_t it = it0; ok && it < it1; ++it) {
       const kvcu_item w = a.items[it];
       const uint32_t end = min(w.end, entry_of(a, w.b, lane == 0).len);
       for (uint32_t p0 = w.start; ok && p0 < end; p0 += ROWS) {
         ++tile;
-        for (uint32_t ch = 0; ok && ch < t.chunks; ++ch)
+        for (uint32_t ch = 0; ok && ch < t.chunks; ++ch) {
+          if (!(ok = wait(B_CE + (unit & 1u), ((unit >> 1) & 1u) ^ 1u))) break;
+          if (lane == 0) {
+            kvtc::mbar_arrive_tx(bar(B_CF + (unit & 1u)), t.width * 16u);
+            bulk_load(base + COL + (unit & 1u) * MAX_N * 16u, t.col + (uint64_t)w.b * t.padded + ch * t.width,
+                      t.width * 16u, bar(B_CF + (unit & 1u)));
+          }
+          __syncwarp();
+          ++unit;
           for (uint32_t u = 0; u < 2 * STAGES; ++u) {  // stage u / 2, part u % 2
             if (!(ok = wait(B_BE + slot, (lap & 1u) ^ 1u))) break;
             // test hook: no copy and no arrival, the waits on it run out
@@ -171,11 +206,16 @@ __global__ void __launch_bounds__(THREADS, 1) k_mass_wide(const __grid_constant_
             }
             if (++slot == t.slots) slot = 0, ++lap;
           }
+        }
       }
     }
     if (!ok) {  // the copies in flight must land before the CTA leaves
       const long long t0 = clock64();
       while (sent && !kvtc::mbar_try(bar(B_BF + lane), (sent - 1) & 1u) && clock64() - t0 <= DRAIN_LIMIT) {
+      }
+      __syncwarp();
+      while (unit && !kvtc::mbar_try(bar(B_CF + ((unit - 1) & 1u)), ((unit - 1) >> 1) & 1u) &&
+             clock64() - t0 <= DRAIN_LIMIT) {
       }
       __syncwarp();
     }
@@ -222,151 +262,137 @@ __global__ void __launch_bounds__(THREADS, 1) k_mass_wide(const __grid_constant_
     const long long t0 = clock64();
     while (!kvtc::mbar_try(bar(B_FINAL), 0) && clock64() - t0 <= DRAIN_LIMIT) {
     }
-  } else if (warp < COMPUTE) {
-    // ---------------------------------------------------------------- rows and sums
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(COMPUTE_REGS));
-    const uint32_t wg = warp >> 2, pair = wg >> 1, half = wg & 1u, r = (warp & 3u) * 32u + lane;
-    const uint32_t lanes = (warp & 3u) * 32u << 16, quarter = t.width / 4, blocks = t.width / 32;
-    const uint32_t ta = tmem + lanes + TM_A + pair * 64u + half * 16u;
+  } else if (warp < DRAIN) {
+    // ---------------------------------------------------------------- sums
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(DRAIN_REGS));
+    const uint32_t g = warp >> 2, r = (warp & 3u) * 32u + lane, half = t.width / 2, blocks = t.width / 32;
+    const uint32_t td = tmem + ((warp & 3u) * 32u << 16) + g * half;
     float* sums = reinterpret_cast<float*>(sm + SUMS) + r;
-    uint32_t x = 0, drained = 0, tiles = 0;  // stages begun by all, groups drained, tiles finished
-    float tot[MAX_BLOCKS][8], run = 0.f;
-    // the unit that the next group to drain belongs to
-    struct Unit {
-      uint32_t b, p, old, c0, flags;  // flags: 1 the row is there, 2 the tile's last chunk
-      float down;                     // the row's power of two, taken back
-    } cur = {}, prev = {};
-    uint32_t cur_first = 0;  // groups before the current unit's
-
-    auto finish = [&](const Unit& u) -> bool {  // the unit's weights; after the last chunk the tile's masses
-      const float4* col = t.col + (uint64_t)u.b * t.padded + u.c0 + wg * quarter;
+    uint32_t group = 0, unit = 0, tiles = 0;  // of the CTA
+    for (uint32_t it = it0; ok && it < it1; ++it) {
+      const kvcu_item w = a.items[it];
+      const Entry e = entry_of(a, w.b, false);
+      const uint32_t end = min(w.end, e.len), old = t.q0 ? e.len : e.old;
+      for (uint32_t p0 = w.start; ok && p0 < end; p0 += ROWS, ++tiles) {
+        const uint32_t p = p0 + r;
+        const uint64_t row = row_of(a, e, p, end, g == 0);
+        const float down = __uint_as_float((254u - scale_of(a, row)) << 23);
+        float* out = a.mass + (uint64_t)w.b * a.mass_stride + p;
+        float run = 0.f, before = 0.f;
+        if (g == 0 && row != NO_ROW && (t.q0 || p < old)) before = *out;
+        for (uint32_t ch = 0; ok && ch < t.chunks; ++ch) {
+          float2 tot[MAX_BLOCKS][8];
+#pragma unroll 1
+          for (uint32_t part = 0; part < STAGES / GROUP; ++part, ++group) {
+            const uint32_t f = group & 1u;
+            if (!(ok = wait(B_DF + f, (group >> 1) & 1u))) break;
+            kvtc::tc_fence_after();
 #pragma unroll
-      for (uint32_t i = 0; i < MAX_BLOCKS; ++i) {
-        if (i >= blocks) continue;
+            for (uint32_t i = 0; i < MAX_BLOCKS; ++i) {
+              if (i >= blocks) continue;
+              uint32_t v[16];
+              kvtc::tmem_ld<16>(td + f * MAX_N + i * 16, v);
+              kvtc::tmem_wait_ld();
+              kvtc::reg_fence(v);
 #pragma unroll
-        for (uint32_t k = 0; k < 8; ++k) {
-          const float4 c = __ldg(col + i * 8 + k);
-          const float w = exp2_approx(fmaf(tot[i][k], c.x * u.down, c.y));
-          run += u.p < __float_as_uint(c.z) ? w : 0.f;
+              for (int k = 0; k < 8; ++k) {
+                const float2 x = make_float2(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1]));
+                tot[i][k] = part ? __fadd2_rn(tot[i][k], x) : x;
+              }
+            }
+            kvtc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) kvtc::mbar_arrive(bar(B_DE + f));
+          }
+          if (!ok) break;
+          if (!(ok = wait(B_CF + (unit & 1u), (unit >> 1) & 1u))) break;
+          const float4* col = reinterpret_cast<const float4*>(sm + COL) + (unit & 1u) * MAX_N + g * half;
+#pragma unroll
+          for (uint32_t i = 0; i < MAX_BLOCKS; ++i) {
+            if (i >= blocks) continue;
+#pragma unroll
+            for (uint32_t k = 0; k < 16; ++k) {
+              const float4 c = col[i * 16 + k];
+              const float weight = exp2_approx(fmaf(k & 1 ? tot[i][k / 2].y : tot[i][k / 2].x, c.x * down, c.y));
+              run += p < __float_as_uint(c.z) ? weight : 0.f;
+            }
+          }
+          __syncwarp();
+          if (lane == 0) kvtc::mbar_arrive(bar(B_CE + (unit & 1u)));
+          ++unit;
+        }
+        if (!ok) break;
+        // the second half's sum to the first, which writes the mass
+        const uint32_t f = tiles & 1u, parity = (tiles >> 1) & 1u;
+        if (g) {
+          if (!(ok = wait(B_SE + f, parity ^ 1u))) break;
+          sums[f * ROWS] = run;
+          __syncwarp();
+          if (lane == 0) kvtc::mbar_arrive(bar(B_SF + f));
+        } else {
+          if (!(ok = wait(B_SF + f, parity))) break;
+          run += sums[f * ROWS];
+          __syncwarp();
+          if (lane == 0) kvtc::mbar_arrive(bar(B_SE + f));
+          if (row != NO_ROW) *out = fmaf(t.q0 ? 1.f : a.decay, before, run);
         }
       }
-      if (!(u.flags & 2u)) return true;
-      const uint32_t f = tiles & 1u, parity = (tiles >> 1) & 1u;
-      if (wg) {
-        if (!wait(B_SE + f, parity ^ 1u)) return false;
-        sums[(f * 3 + wg - 1) * ROWS] = run;
-        __syncwarp();
-        if (lane == 0) kvtc::mbar_arrive(bar(B_SF + f));
-      } else {
-        float* out = a.mass + (uint64_t)u.b * a.mass_stride + u.p;
-        const float before = (u.flags & 1u) && (t.q0 || u.p < u.old) ? *out : 0.f;
-        if (!wait(B_SF + f, parity)) return false;
-#pragma unroll
-        for (int k = 0; k < 3; ++k) run += sums[(f * 3 + k) * ROWS];
-        __syncwarp();
-        if (lane == 0) kvtc::mbar_arrive(bar(B_SE + f));
-        if (u.flags & 1u) *out = fmaf(t.q0 ? 1.f : a.decay, before, run);
-      }
-      run = 0.f;
-      ++tiles;
-      return true;
-    };
-    // the sums of the oldest group that was not taken yet
-    auto drain = [&]() -> bool {
-      const uint32_t f = drained & 1u, part = drained % (STAGES / GROUP);
-      if (!wait(B_DF + f, (drained >> 1) & 1u)) return false;
-      kvtc::tc_fence_after();
-      const uint32_t td = tmem + lanes + f * MAX_N + wg * quarter;
-#pragma unroll
-      for (uint32_t i = 0; i < MAX_BLOCKS; ++i) {
-        if (i >= blocks) continue;
-        uint32_t v[8];
-        kvtc::tmem_ld<8>(td + i * 8, v);
-        kvtc::tmem_wait_ld();
-        kvtc::reg_fence(v);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) tot[i][k] = part ? tot[i][k] + __uint_as_float(v[k]) : __uint_as_float(v[k]);
-      }
-      kvtc::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) kvtc::mbar_arrive(bar(B_DE + f));
-      const bool of_prev = drained < cur_first;
-      ++drained;
-      return part != STAGES / GROUP - 1 || finish(of_prev ? prev : cur);
-    };
-
+    }
+  } else if (warp < UNPACK) {
+    // ---------------------------------------------------------------- rows
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(UNPACK_REGS));
+    const uint32_t pair = (warp - DRAIN) >> 2, r = (warp & 3u) * 32u + lane;
+    const uint32_t ta = tmem + ((warp & 3u) * 32u << 16) + TM_A + pair * 64u;
+    uint32_t x = 0;  // stages of the units before
     for (uint32_t it = it0; ok && it < it1; ++it) {
       const kvcu_item w = a.items[it];
       const Entry e = entry_of(a, w.b, false);
       const uint32_t end = min(w.end, e.len);
       for (uint32_t p0 = w.start; ok && p0 < end; p0 += ROWS) {
-        const uint32_t p = p0 + r, blk = p < end ? a.tables[e.t0 + p / a.block_size] : 0xFFFFFFFFu;
-        const bool good = blk < a.num_blocks;
-        if (p < end && !good) atomicOr(a.status, KVCU_STATUS_BAD_BLOCK);
-        const uint64_t row = good ? ((uint64_t)a.layer * a.num_blocks + blk) * a.block_size + p % a.block_size : 0;
-        const uint4* values = reinterpret_cast<const uint4*>(a.qs + row * W + half * 32u);
+        const uint64_t row = row_of(a, e, p0 + r, end, false);
+        const float up = __uint_as_float(scale_of(a, row) << 23);
+        const uint4* values = reinterpret_cast<const uint4*>(a.qs + row * W);
         const uint32_t* scales = reinterpret_cast<const uint32_t*>(a.sc + row * NBLK);  // rows are 36 bytes
-        // the power of two that brings the largest scale to [2^7, 2^8)
-        uint32_t top = 0;
-#pragma unroll
-        for (uint32_t s = 0; s < STAGES; ++s) {
-          const uint32_t two = good ? __ldg(scales + s) & 0x7fff7fffu : 0u;
-          top = max(top, max(two & 0xffffu, two >> 16));
-        }
-        const uint32_t tf = __float_as_uint(__half2float(__ushort_as_half((unsigned short)top)));
-        const uint32_t field = top == 0u || top >= 0x7c00u ? 127u : 261u - (tf >> 23);  // 2^(7 - exponent)
-        const float up = __uint_as_float(field << 23), down = __uint_as_float((254u - field) << 23);
-        uint32_t s = (x ^ pair) & 1u;  // this pair's first stage
-        uint4 d0 = {}, d1 = {};
+        uint4 d[4] = {};
         uint32_t sc = 0;
-        auto load = [&](uint32_t at) {
-          if (!good) return;
-          d0 = __ldg(values + at * 4);
-          d1 = __ldg(values + at * 4 + 1);
-          sc = __ldg(scales + at);
-        };
-        load(s);
-        for (uint32_t ch = 0; ok && ch < t.chunks; ++ch) {
-          prev = cur;
-          cur = {w.b, p, t.q0 ? e.len : e.old, ch * t.width, (good ? 1u : 0u) | (ch + 1 == t.chunks ? 2u : 0u), down};
-          cur_first = x / GROUP;
-          for (s = (x ^ pair) & 1u; s < STAGES; s += 2) {
-            const uint32_t at = x + s;  // of all stages; this pair's buffer's (at >> 1)-th
-            if (!(ok = wait(B_AE + pair, ((at >> 1) & 1u) ^ 1u))) break;
-            const __half one = __float2half_rn(__half2float(__ushort_as_half((unsigned short)(half ? sc >> 16 : sc & 0xffffu))) * up);
-            const __half2 scale = __half2half2(one);
-            auto part = [&](uint4 v, uint32_t to) {  // 16 values: eight columns of each part
-              uint32_t h[8], hi[8], lo[8];
-              int8_to_f16(v.x, h);
-              int8_to_f16(v.y, h + 2);
-              int8_to_f16(v.z, h + 4);
-              int8_to_f16(v.w, h + 6);
+        auto load = [&](uint32_t s) {
+          if (row == NO_ROW) return;
 #pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                const __half2 y = *reinterpret_cast<const __half2*>(&h[k]), top = __hmul2_rn(y, scale);
-                const __half2 rest = __hfma2(y, scale, __hneg2(top));
-                hi[k] = *reinterpret_cast<const uint32_t*>(&top);
-                lo[k] = *reinterpret_cast<const uint32_t*>(&rest);
+          for (int k = 0; k < 4; ++k) d[k] = __ldg(values + s * 4 + k);
+          sc = __ldg(scales + s);
+        };
+        load((x ^ pair) & 1u);
+        for (uint32_t ch = 0; ok && ch < t.chunks; ++ch, x += STAGES)
+          for (uint32_t s = (x ^ pair) & 1u; s < STAGES; s += 2) {
+            // this pair's buffer's n-th use
+            if (!(ok = wait(B_AE + pair, (((x + s) >> 1) & 1u) ^ 1u))) break;
+            const float2 both = __half22float2(*reinterpret_cast<const __half2*>(&sc));
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {  // 16 values: eight columns of each part
+              const __half2 scale = __float2half2_rn((k < 2 ? both.x : both.y) * up);
+              uint32_t y[8], lo[8];
+              int8_to_f16(d[k].x, y);
+              int8_to_f16(d[k].y, y + 2);
+              int8_to_f16(d[k].z, y + 4);
+              int8_to_f16(d[k].w, y + 6);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const __half2 v = *reinterpret_cast<const __half2*>(&y[i]), top = __hmul2_rn(v, scale);
+                const __half2 rest = __hfma2(v, scale, __hneg2(top));
+                y[i] = *reinterpret_cast<const uint32_t*>(&top);
+                lo[i] = *reinterpret_cast<const uint32_t*>(&rest);
               }
-              kvtc::tmem_st<8>(to, hi);
-              kvtc::tmem_st<8>(to + 32, lo);
-            };
-            part(d0, ta);
-            part(d1, ta + 8);
-            load(s + 2 < STAGES ? s + 2 : (s + 2) - STAGES);  // the next one of this tile, if there is one
+              kvtc::tmem_st<8>(ta + k * 8, y);
+              kvtc::tmem_st<8>(ta + 32 + k * 8, lo);
+            }
+            load(s + 2 < STAGES ? s + 2 : s + 2 - STAGES);  // the next one of this tile, if there is one
             kvtc::tmem_wait_st();
             kvtc::tc_fence_before();
             __syncwarp();
             if (lane == 0) kvtc::mbar_arrive(bar(B_AF + pair));
-            // groups whose MMAs are over: those up to the stage whose buffer was free just now
-            while (ok && GROUP * (drained + 1) + 1 <= at) ok = drain();
-            if (!ok) break;
           }
-          x += STAGES;
-        }
       }
     }
-    while (ok && GROUP * (drained + 1) <= x) ok = drain();
   }
   // ---- teardown
   kvcu_pdl_trigger();
