@@ -561,6 +561,36 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   }
 }
 
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// Boxes of `box_cols` x `box_rows` elements of a row-major [rows][width] array; 64B swizzle for
+// 64-byte boxes, else 128B.
+int make_map(CUtensorMap* map, CUtensorMapDataType type, uint32_t elt, const void* at, uint64_t rows, uint32_t width,
+             uint32_t box_cols, uint32_t box_rows) {
+  static EncodeTiledFn enc = []() -> EncodeTiledFn {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return nullptr;
+    return reinterpret_cast<EncodeTiledFn>(f);
+  }();
+  if (!enc) {
+    kvcu_set_error("cuTensorMapEncodeTiled unavailable");
+    return KVCU_ERR_CUDA;
+  }
+  const cuuint64_t dims[2] = {width, rows}, strides[1] = {(cuuint64_t)width * elt};
+  const cuuint32_t estr[2] = {1, 1}, boxes[2] = {box_cols, box_rows};
+  const CUresult r = enc(map, type, 2, const_cast<void*>(at), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         box_cols * elt == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r == CUDA_SUCCESS) return KVCU_OK;
+  kvcu_set_error("cuTensorMapEncodeTiled failed: %d", (int)r);
+  return KVCU_ERR_CUDA;
+}
+
 // Boxes of 128-byte pieces of the rows: Q8_0 bytes 0 .. 511 and the last 64; f32 latents and rope parts.
 int make_maps(const kvcu_pool* p, uint32_t box_rows, CUtensorMap* wide, CUtensorMap* tail) {
   const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8, f32 = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
@@ -626,38 +656,6 @@ struct DevScope {
 };
 
 }  // namespace
-
-namespace kvmass {
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-int make_map(CUtensorMap* map, CUtensorMapDataType type, uint32_t elt, const void* at, uint64_t rows, uint32_t width,
-             uint32_t box_cols, uint32_t box_rows) {
-  static EncodeTiledFn enc = []() -> EncodeTiledFn {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      return nullptr;
-    return reinterpret_cast<EncodeTiledFn>(f);
-  }();
-  if (!enc) {
-    kvcu_set_error("cuTensorMapEncodeTiled unavailable");
-    return KVCU_ERR_CUDA;
-  }
-  const cuuint64_t dims[2] = {width, rows}, strides[1] = {(cuuint64_t)width * elt};
-  const cuuint32_t estr[2] = {1, 1}, boxes[2] = {box_cols, box_rows};
-  const CUresult r = enc(map, type, 2, const_cast<void*>(at), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         box_cols * elt == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
-                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r == CUDA_SUCCESS) return KVCU_OK;
-  kvcu_set_error("cuTensorMapEncodeTiled failed: %d", (int)r);
-  return KVCU_ERR_CUDA;
-}
-
-}  // namespace kvmass
 
 extern "C" int kvcu_attn_mass(kvcu_decode_ws* ws, kvcu_pool* pool, uint32_t layer, uint32_t n, const uint32_t* seq_ids,
                               uint32_t n_seqs, const uint32_t* table_offsets, const uint32_t* tables,

@@ -147,11 +147,6 @@ __device__ __forceinline__ uint32_t scale_field(uint32_t top) {
   return top == 0u || eb >= 255u ? 127u : (uint32_t)min(max(267 - (int)eb, 1), 253);
 }
 
-// Boxes of `box_cols` x `box_rows` elements of a row-major [rows][width] array, 128B
-// swizzle for 128-byte boxes, 64B for 64-byte ones (kvcu_mass.cu).
-int make_map(CUtensorMap* map, CUtensorMapDataType type, uint32_t elt, const void* at, uint64_t rows, uint32_t width,
-             uint32_t box_cols, uint32_t box_rows);
-
 // The kernel for many columns (kvcu_mass_wide.cu): queries [q0, q0 + count) of every entry.
 constexpr uint32_t WIDE_MIN_COLS = 64;
 uint64_t wide_scratch(uint32_t n, uint32_t cols);  // bytes it takes for n entries of `cols` columns

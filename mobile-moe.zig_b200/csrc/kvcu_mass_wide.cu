@@ -20,7 +20,7 @@
 //                exponentials, and the row's mass
 //   warps 8-15   unpack: each thread one row's 64 values of every second stage, to f16
 //                parts in the stage's TMEM buffer
-//   warp 16      producer: TMA boxes of 64 elements x N columns of one part
+//   warp 16      producer: bulk copies of 64 elements of N columns of one part, laid out for the MMA
 //   warp 17      issues the MMAs
 #include "kvcu_mass.cuh"
 
@@ -51,6 +51,7 @@ struct Wide {
   MassArgs m;
   uint32_t q0, cols, chunks, width, padded;  // of an entry: first query, columns, chunks of `width`, chunks * width
   uint32_t slots;                            // of the ring
+  const char* parts;
   const float4* col;                         // [n][padded]: scale, -lse, limit (bits)
   long long wait_limit;
   uint32_t withhold_plus1;  // test hook: 0, or 1 + the tile of each CTA whose first unit of B is withheld
@@ -84,8 +85,9 @@ __device__ __forceinline__ uint32_t scale_of(const MassArgs& a, uint64_t row) {
   return top == 0u || top >= 0x7c00u ? 127u : 261u - (bits >> 23);  // 7 - exponent, biased
 }
 
-// The columns' parts, [n][hi, lo][padded][W] f16, and constants; a warp to a column.
-__global__ void __launch_bounds__(256) k_mass_wide_q(const Wide t, __half* parts, float4* consts) {
+// The columns' parts, [n][chunk][stage][hi, lo] units of B as shared memory holds them (`width`
+// rows of 64 f16, 128B swizzle), and constants; a warp to a column.
+__global__ void __launch_bounds__(256) k_mass_wide_q(const Wide t, char* parts, float4* consts) {
   kvcu_pdl_wait();
   const MassArgs& a = t.m;
   const uint64_t id = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -106,8 +108,7 @@ __global__ void __launch_bounds__(256) k_mass_wide_q(const Wide t, __half* parts
   }
   const uint32_t field = scale_field(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
   const float up = __uint_as_float(field << 23);
-  uint2* hi = reinterpret_cast<uint2*>(parts + ((uint64_t)b * 2 * t.padded + c) * W);
-  uint2* lo = hi + (uint64_t)t.padded * (W / 4);
+  char* units = parts + ((uint64_t)b * t.chunks + c / t.width) * STAGES * 2 * (t.width * 128u);
 #pragma unroll
   for (int k = 0; k < 5; ++k) {
     const uint32_t f = lane + 32 * k;
@@ -115,8 +116,9 @@ __global__ void __launch_bounds__(256) k_mass_wide_q(const Wide t, __half* parts
     uint2 h, l;
     split(x[k].x * up, x[k].y * up, &h.x, &l.x);
     split(x[k].z * up, x[k].w * up, &h.y, &l.y);
-    hi[f] = h;
-    lo[f] = l;
+    char* to = units + f / 16 * 2 * (t.width * 128u) + kvtc::sw128_off(c % t.width, f % 16 * 8);
+    *reinterpret_cast<uint2*>(to) = h;
+    *reinterpret_cast<uint2*>(to + t.width * 128u) = l;
   }
   if (lane == 0) {
     constexpr double LOG2E = 1.4426950408889634;
@@ -129,7 +131,7 @@ __global__ void __launch_bounds__(256) k_mass_wide_q(const Wide t, __half* parts
   }
 }
 
-__global__ void __launch_bounds__(THREADS, 1) k_mass_wide(const __grid_constant__ CUtensorMap map, const Wide t) {
+__global__ void __launch_bounds__(THREADS, 1) k_mass_wide(const Wide t) {
   const MassArgs& a = t.m;
   extern __shared__ char raw[];
   char* sm = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -198,8 +200,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_mass_wide(const __grid_constant_
             if (!(u == 0 && ch == 0 && tile == t.withhold_plus1)) {
               if (lane == 0) {
                 kvtc::mbar_arrive_tx(bar(B_BF + slot), unit_bytes);
-                tma_2d(base + slot * unit_bytes, &map, (int)(u / 2 * 64),
-                       (int)((w.b * 2 + (u & 1u)) * t.padded + ch * t.width), bar(B_BF + slot));
+                bulk_load(base + slot * unit_bytes,
+                          t.parts + (((uint64_t)w.b * t.chunks + ch) * STAGES * 2 + u) * unit_bytes, unit_bytes,
+                          bar(B_BF + slot));
               }
               __syncwarp();
               sent += lane == slot;
@@ -427,8 +430,9 @@ int launch_wide(const kvcu_pool* pool, const MassArgs& a, uint32_t q0, uint32_t 
   t.slots = RING_BYTES / (t.width * 128u);
   if (t.slots > MAX_SLOTS) t.slots = MAX_SLOTS;
   const uint64_t columns = (uint64_t)a.n * t.padded;
-  __half* parts = static_cast<__half*>(scratch);
-  float4* consts = reinterpret_cast<float4*>(parts + columns * 2 * W);
+  char* parts = static_cast<char*>(scratch);
+  float4* consts = reinterpret_cast<float4*>(parts + columns * 2 * W * sizeof(__half));
+  t.parts = parts;
   t.col = consts;
   t.wait_limit = ws->wait_limit ? (long long)ws->wait_limit : (1ll << 31);
   t.withhold_plus1 = ws->withhold_plus1;
@@ -448,13 +452,10 @@ int launch_wide(const kvcu_pool* pool, const MassArgs& a, uint32_t q0, uint32_t 
       },
       nullptr);
   if (rc) return rc;
-  CUtensorMap map;
-  rc = make_map(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, parts, 2 * columns, W, 64, t.width);
-  if (rc) return rc;
   rc = kvcu_check_cuda(kvcu_launch_pdl(k_mass_wide_q, dim3((uint32_t)((columns + 7) / 8)), dim3(256), 0, st, t, parts, consts),
                        "attention mass columns launch");
   if (rc) return rc;
-  return kvcu_check_cuda(kvcu_launch_pdl(k_mass_wide, dim3((uint32_t)ws->decode_ctas), dim3(THREADS), ALLOC, st, map, t),
+  return kvcu_check_cuda(kvcu_launch_pdl(k_mass_wide, dim3((uint32_t)ws->decode_ctas), dim3(THREADS), ALLOC, st, t),
                          "attention mass launch");
 }
 
