@@ -5,7 +5,7 @@
 // chunks re-unpack the rows.  Here a row's value, int8 times its block's scale (19 bits),
 // is the exact sum of two f16 parts, so one accumulator serves all of K = 576: a GEMM
 //   S[row][column] = A_hi B_hi + A_lo B_hi + A_hi B_lo       (low times low < 2^-22)
-// with 128 rows to a tile (A, unpacked into TMEM), up to 96 columns to a chunk (B, q's
+// with 128 rows to a tile (A, unpacked into TMEM), up to 128 columns to a chunk (B, q's
 // parts made by k_mass_wide_q) and the exponentials as its epilogue.
 //   A row's scales are brought to at most 2^8 by a power of two of the row; its parts
 // are exact for blocks with scales down to 2^-21 of the row's largest, and within
@@ -32,22 +32,22 @@ namespace {
 
 constexpr int DRAIN = 8, UNPACK = 16, PRODUCER = 16, ISSUER = 17, THREADS = 20 * 32;  // warps up to DRAIN, UNPACK
 // Registers: launched with 96 a thread; the last warpgroup gives to the others.
-constexpr int LAUNCH_REGS = 96, DRAIN_REGS = 104, UNPACK_REGS = 104, SERVICE_REGS = 64;
+constexpr int LAUNCH_REGS = 96, DRAIN_REGS = 120, UNPACK_REGS = 88, SERVICE_REGS = 64;
 static_assert(8 * DRAIN_REGS + 8 * UNPACK_REGS + 4 * SERVICE_REGS <= 20 * LAUNCH_REGS,
               "register split exceeds the launch allocation");
-static_assert(DRAIN_REGS > LAUNCH_REGS && UNPACK_REGS > LAUNCH_REGS && SERVICE_REGS < LAUNCH_REGS,
+static_assert(DRAIN_REGS > LAUNCH_REGS && UNPACK_REGS < LAUNCH_REGS && SERVICE_REGS < LAUNCH_REGS,
               "an increase to fewer registers, or a decrease to more, is an illegal instruction");
 constexpr uint32_t ROWS = 128, STAGES = W / 64;
-constexpr uint32_t MAX_N = 96, MAX_BLOCKS = MAX_N / 32;  // columns of a chunk; blocks of 16 a thread drains
+constexpr uint32_t MAX_N = 128, MAX_BLOCKS = MAX_N / 32;  // columns of a chunk; blocks of 16 a thread drains
 constexpr uint32_t COL_BYTES = 12;  // constants of a column: scale and -lse, two columns' to 16 bytes; then the limits
 constexpr uint32_t GROUP = 3;                             // stages to a drain
-constexpr uint32_t RING_BYTES = 16 * MAX_N * 128, SLOTS = 16;  // of the ring: high parts in the even ones
-constexpr uint32_t TM_X = 2 * MAX_N, TM_A = 4 * MAX_N, TM_COLS = 512;  // TMEM: two main sums, two of the low parts', two stages of 64
+constexpr uint32_t RING_BYTES = 12 * MAX_N * 128, SLOTS = 12;  // of the ring: high parts in the even ones
+constexpr uint32_t TM_X = 2 * MAX_N, TM_A = 3 * MAX_N, TM_COLS = 512;  // TMEM: two main sums, the low parts', two stages of 64
 constexpr uint32_t COL = RING_BYTES;  // [2] a chunk's constants
 constexpr uint32_t SUMS = COL + 2 * MAX_N * COL_BYTES;                // [2][ROWS]
 // barriers
 constexpr int B_BF = 0, B_BE = SLOTS, B_AF = 2 * SLOTS, B_AE = B_AF + 2, B_DF = B_AE + 2, B_DE = B_DF + 2,
-              B_SF = B_DE + 2, B_SE = B_SF + 2, B_CF = B_SE + 2, B_CE = B_CF + 2, B_XF = B_CE + 2, B_XE = B_XF + 2, B_FINAL = B_XE + 2, NUM_BARS = B_FINAL + 1;
+              B_SF = B_DE + 2, B_SE = B_SF + 2, B_CF = B_SE + 2, B_CE = B_CF + 2, B_XF = B_CE + 2, B_XE = B_XF + 1, B_FINAL = B_XE + 1, NUM_BARS = B_FINAL + 1;
 constexpr uint32_t BARS = SUMS + 2 * ROWS * 4, MISC = BARS + NUM_BARS * 8, ALLOC = MISC + 16 + 1024;
 static_assert(ALLOC <= 232448 && TM_A + 2 * 64 <= TM_COLS, "budgets");
 constexpr long long DRAIN_LIMIT = 1ll << 31;
@@ -172,8 +172,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_mass_wide(const Wide t) {
     init(B_SE, 2, 4);
     init(B_CF, 2, 1);
     init(B_CE, 2, DRAIN);
-    init(B_XF, 2, 1);
-    init(B_XE, 2, DRAIN);
+    init(B_XF, 1, 1);
+    init(B_XE, 1, DRAIN);
     init(B_FINAL, 1, 2);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -256,9 +256,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_mass_wide(const Wide t) {
       const uint32_t end = min(w.end, entry_of(a, w.b, false).len);
       const uint32_t units = w.start < end ? (end - w.start + ROWS - 1) / ROWS * t.chunks : 0u;
       for (uint32_t s = 0; s < units * STAGES; ++s, ++x) {
-        const uint32_t period = main ? GROUP : STAGES, n = x / period, f = n & 1u;
+        const uint32_t period = main ? GROUP : STAGES, n = x / period, f = main ? n & 1u : 0u;
         const bool first = x % period == 0, last = x % period == period - 1;
-        if (first && !(ok = wait((main ? B_DE : B_XE) + f, ((n >> 1) & 1u) ^ 1u))) break;
+        if (first && !(ok = wait((main ? B_DE : B_XE) + f, ((main ? n >> 1 : n) & 1u) ^ 1u))) break;
         if (!(ok = wait(B_AF + (x & 1u), (x >> 1) & 1u)) || !(ok = wait(B_BF + slot, lap & 1u))) break;
         const uint32_t td = tmem + (main ? 0u : TM_X) + f * MAX_N, ta = tmem + TM_A + (x & 1u) * 64u;
         const uint64_t hi = kvtc::smem_desc(base + slot * unit_bytes, 16, 1024, kvtc::LAYOUT_SW128);
@@ -339,17 +339,19 @@ __global__ void __launch_bounds__(THREADS, 1) k_mass_wide(const Wide t) {
                 }
               }
             };
+            auto done = [&](uint32_t i) {
+              kvtc::tc_fence_before();
+              __syncwarp();
+              if (lane == 0) kvtc::mbar_arrive(bar(i));
+            };
+            if (part == STAGES / GROUP - 1) {  // the low parts' first: there is one accumulator of them
+              if (!(ok = wait(B_XF, unit & 1u))) break;
+              kvtc::tc_fence_after();
+              take(td + TM_X, false);
+              done(B_XE);
+            }
             take(td + f * MAX_N, part == 0);
-            kvtc::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) kvtc::mbar_arrive(bar(B_DE + f));
-            if (part < STAGES / GROUP - 1) continue;
-            if (!(ok = wait(B_XF + (unit & 1u), (unit >> 1) & 1u))) break;
-            kvtc::tc_fence_after();
-            take(td + TM_X + (unit & 1u) * MAX_N, false);
-            kvtc::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) kvtc::mbar_arrive(bar(B_XE + (unit & 1u)));
+            done(B_DE + f);
           }
           if (!ok) break;
           if (!(ok = wait(B_CF + (unit & 1u), (unit >> 1) & 1u))) break;
@@ -403,7 +405,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_mass_wide(const Wide t) {
     }
   } else if (warp < UNPACK) {
     // ---------------------------------------------------------------- rows
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(UNPACK_REGS));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(UNPACK_REGS));
     const uint32_t pair = (warp - DRAIN) >> 2, r = (warp & 3u) * 32u + lane, piece = lane & 3u;
     const uint32_t ta = tmem + ((warp & 3u) * 32u << 16) + TM_A + pair * 64u;
     uint32_t x = 0;  // stages of the units before
