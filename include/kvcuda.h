@@ -369,7 +369,10 @@ int kvcu_mla_decode_noalloc(kvcu_pool* pool, uint32_t layer, uint32_t n, const u
  * KVCU_STATUS_BAD_LEN and is cut, a bad block sets KVCU_STATUS_BAD_BLOCK and its
  * positions are left.  Entries may share a sequence (each has its own sums).
  * Runs on the last one-layer plan of `ws` (kvcu_decode_plan or _causal; the
- * batch must be the one planned), so a step's decode and its mass share it. */
+ * batch must be the one planned), so a step's decode and its mass share it; for
+ * many columns (n_q * n_heads) of Q8_0 rows it also uses the workspace's decode
+ * partials, so as with decodes, calls that share a workspace belong on one stream.
+ * After KVCU_STATUS_TIMEOUT the sums are undefined. */
 int kvcu_attn_mass(kvcu_decode_ws* ws, kvcu_pool* pool, uint32_t layer, uint32_t n, const uint32_t* seq_ids,
                    uint32_t n_seqs, const uint32_t* table_offsets, const uint32_t* tables, const uint32_t* lens,
                    uint32_t n_q, const float* q, const float* lse, uint32_t n_heads, float scale, float decay,

@@ -119,11 +119,12 @@ int kvcu_init(int device) {
     kvcu_set_error("kvcu_init: device %d out of range [0, %d)", device, n);
     return KVCU_ERR_INVALID_ARG;
   }
-  cudaDeviceProp prop;
-  KVCU_CUDA(cudaGetDeviceProperties(&prop, device));
-  if (prop.major != 10) {
-    kvcu_set_error("kvcu_init: device %d is sm_%d%d; this library is built for sm_100a (B200)",
-                   device, prop.major, prop.minor);
+  // two attributes: reading all properties takes about a millisecond
+  int major = 0, minor = 0;
+  KVCU_CUDA(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device));
+  KVCU_CUDA(cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, device));
+  if (major != 10) {
+    kvcu_set_error("kvcu_init: device %d is sm_%d%d; this library is built for sm_100a (B200)", device, major, minor);
     return KVCU_ERR_UNSUPPORTED;
   }
   DeviceGuard g(device);
