@@ -629,7 +629,7 @@ int kvcache_mla_step_dev(kvcache* c, uint32_t layer, uint32_t n, const uint32_t*
  * The step above with the rotary frequencies of `rope` at rope_positions[b] (host;
  * NULL: the cache positions): in a cache that evicts, a token's position runs on
  * while its row goes to the next free place.  q_abs_dev [n][H][R+P] and lse_dev
- * [n][H] (device, each may be NULL) receive the absorbed queries and the
+ * [n][H] (device, each may be NULL; q_abs_dev 16-byte aligned) receive the absorbed queries and the
  * log-sum-exp of the scaled scores over the history and the newest token, what
  * kvcache_attn_mass_dev takes. */
 int kvcache_mla_step_rope_dev(kvcache* c, uint32_t layer, uint32_t n, const uint32_t* seq_ids,
@@ -659,7 +659,8 @@ int kvcache_attn_mass_dev(kvcache* c, uint32_t layer, uint32_t n, const uint32_t
  * blocks behind return to the pool, as after a truncate.  Blocks held elsewhere
  * (a shared prefix, a running save) are copied before rows move into them
  * (KVCU_ERR_OUT_OF_BLOCKS where none is free; nothing is evicted then), and
- * rewritten blocks leave the prefix cache.  keep_dev (device, may be NULL)
+ * rewritten blocks leave the prefix cache (and must not be entered again: their
+ * rows are no longer those of consecutive tokens).  keep_dev (device, may be NULL)
  * receives the kept positions [n_layers][n][budget].  Call it between steps,
  * when every layer holds the sequences' rows, ordered after the calls that
  * wrote or read them; the cache's next append, step, decode or gather, on any

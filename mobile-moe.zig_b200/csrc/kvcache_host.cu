@@ -1346,6 +1346,10 @@ int kvcache_mla_step_rope_dev(kvcache* c, uint32_t layer, uint32_t n, const uint
                    c ? c->rope_dim : 0u);
     return KVCU_ERR_INVALID_ARG;
   }
+  if ((uintptr_t)q_abs_dev & 15u) {
+    kvcu_set_error("kvcache_mla_step_rope_dev: the absorbed queries are not 16-byte aligned");
+    return KVCU_ERR_INVALID_ARG;
+  }
   return guarded("kvcache_mla_step_rope_dev", [&] {
     return step_impl(c, layer, n, seq_ids, positions, rope, rope_positions, q_dev, kv_a_dev, norm_w_dev, eps, 0.0f,
                      k_b_dev, v_b_dev, n_heads, qk_nope, v_dim, scale, attn_dev, q_abs_dev, lse_dev, stream);

@@ -369,11 +369,15 @@ __global__ void __launch_bounds__(THREADS, 1) k_mass_wide(const Wide t) {
               use(i * 8 + k, make_float2(exp2_approx(s.x), exp2_approx(s.y)));
             }
           };
+          const float2 start = run;
           if (inside) {
 #pragma unroll
             for (uint32_t i = 0; i < MAX_BLOCKS; ++i)
               if (i < blocks) weigh(i, [&](uint32_t, float2 weight) { run = __fadd2_rn(run, weight); });
-          } else {
+          }
+          // also for a row whose infinities or NaN met a column without positions (0 times them is NaN)
+          if (!inside || !(run.x + run.y < INFINITY)) {
+            run = start;
 #pragma unroll
             for (uint32_t i = 0; i < MAX_BLOCKS; ++i)
               if (i < blocks)

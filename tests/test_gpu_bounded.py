@@ -427,8 +427,16 @@ def test_refusals(kv):
         c.attnMass_dev(0, [0, 1], q, lse, SCALE, row)
     with pytest.raises(ValueError):
         c.attnMass_dev(0, [0], q, lse[:, :19], SCALE, row)
+    with pytest.raises(ValueError):
+        c.attnMass_dev(0, [0], q[..., :512].contiguous(), lse, SCALE, row)
+    with pytest.raises(ValueError):
+        c.mlaDecodeLse_dev(0, [0], q, SCALE, torch.zeros(1, H, R, device="cuda"), lse[:, :19])
+    with pytest.raises(ValueError):
+        c.evict_dev([0, 1], 64, mass.double())
     st = Step(1, 1)
     refused("InvalidArgument", st.run, c, 0, [1], [40], kv.Rope(32))   # another rotary part than the cache's
     refused("PositionOutOfBounds", st.run, c, 0, [1], [200], kv.Rope(P))
+    st.q_abs = torch.zeros(H * W + 1, device="cuda")[1:].view(1, H, W)
+    refused("InvalidArgument", st.run, c, 0, [1], [40], kv.Rope(P))    # not 16-byte aligned
     with pytest.raises(ValueError):
         st.run(c, 0, [1], [40], kv.Rope(P), rope_pos=[1, 2])

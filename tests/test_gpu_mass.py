@@ -308,6 +308,12 @@ def test_refusals(kv):
     shifted = torch.zeros(2 * 20 * W + 1, device="cuda")[1:].view(2, 1, 20, W)
     with pytest.raises(kv.KVCudaError):  # q not 16-byte aligned
         ws.attn_mass(cache.pool, 0, shifted, lse, *args, mass)
+    with pytest.raises(ValueError):  # queries of another width than the rows
+        ws.attn_mass(cache.pool, 0, q[..., :512].contiguous(), lse, *args, mass)
+    with pytest.raises(ValueError):
+        ws.attn_mass(cache.pool, 0, q.half(), lse, *args, mass)
+    with pytest.raises(ValueError):
+        ws.attn_mass(cache.pool, 0, q, lse, cache.toff, cache.tables, cache.lens_dev.long(), SCALE, mass)
     ws.plan_layers(cache.pool, cache.lens_dev, 2)
     with pytest.raises(kv.KVCudaError):  # a layered plan
         ws.attn_mass(cache.pool, 0, q, lse, *args, mass)
@@ -392,6 +398,31 @@ def test_many_columns_withheld_and_again(kv):
     ws.test_withhold(0xFFFFFFFF)
     ws.set_wait_limit(0)
     assert torch.equal(run(), want) and cache.pool.status() == 0
+
+
+@pytest.mark.parametrize("n_q", [1, 4])
+def test_nan_rows_and_queries_without_positions(kv, n_q):
+    """Queries with lse = -inf add nothing, also to rows of NaN and infinities; a live query's NaN shows
+    in the rows that have them and in no other."""
+    import torch
+
+    from pooldata import arrays
+
+    cache = Paged(kv, [300, 1000], 64, True, seed=14)
+    q, lse = queries(cache, range(2), n_q, 20, 6)
+    _, sc = arrays(cache.pool)
+    for s, value in ((0, float("nan")), (1, float("inf"))):
+        sc[torch.from_numpy(cache.rows_at(s, [3, 130])).cuda()] = value
+    lse[0] = -math.inf
+    mass = torch.rand(2, 1000, device="cuda")
+    before = mass.clone()
+    ws = kv.DecodeWorkspace(0, 2, 20)
+    ws.plan(cache.pool, cache.lens_dev)
+    ws.attn_mass(cache.pool, 0, q, lse, cache.toff, cache.tables, cache.lens_dev, SCALE, mass, decay=0.5)
+    assert torch.equal(mass[0, :300], before[0, :300] * 0.5) and torch.equal(mass[0, 300:], before[0, 300:])
+    fine = torch.ones(1000, dtype=torch.bool, device="cuda")
+    fine[[3, 130]] = False
+    assert torch.isfinite(mass[1, fine]).all() and not torch.isfinite(mass[1, ~fine]).any()
 
 
 @pytest.mark.parametrize("quant", [True, False])
