@@ -6,7 +6,7 @@
 //   masses' 32-bit order (11 + 11 + 10 bits): the row is read once into shared
 //   memory while the first histogram is formed, the other passes run there.
 //   Floor: one read of the masses (4 B per position); bound: the instructions of three
-//   passes.  512 rows of 1.5k to 65k positions, 2,048 kept: 59 us (35.9 MB read once).
+//   passes.  512 rows of 1.5k to 65k positions, 2,048 kept: 57 us (35.9 MB read once).
 // k_evict_compact: row j of a sequence := its row keep[j], in place through the
 //   block table, in every layer, and the masses with it.  Bound: one read and
 //   one write of the kept rows.  512 pairs of 2,048 rows of 612 B: 252 us, 4.3 TB/s.
@@ -155,6 +155,10 @@ __global__ void __launch_bounds__(NT, 2) k_evict_select(SelectArgs a) {
     return make_uint4(order_key(x.x), order_key(x.y), order_key(x.z), order_key(x.w));
   };
   auto keys_at = [&](uint32_t g) -> uint4 { return g < a.cap ? cache[g] : keys_of(read(g)); };
+  auto whole = [&](uint32_t g) {
+    const uint32_t v = 4 * g - off;
+    return v < cnt && v + 4 <= cnt;
+  };
   // f(key, position in the share) for the group's positions that are there
   auto each = [&](uint32_t g, const uint4& k, auto&& f) {
     const uint32_t v = 4 * g - off;
@@ -215,16 +219,24 @@ __global__ void __launch_bounds__(NT, 2) k_evict_select(SelectArgs a) {
             if (g0 + j * 32 < w1) k[j] = keys_at(g0 + j * 32);
 #pragma unroll
           for (uint32_t j = 0; j < U; ++j)
-            if (g0 + j * 32 < w1)
-              each(g0 + j * 32, k[j], [&](uint32_t v, uint32_t at) {
-                if (v < lo) return;
-                if (v - lo >= 1u << 21) {
-                  ++sure;
-                } else {
-                  const uint32_t n = atomicAdd(&s_listed, 1u);
-                  if (n < LIST) list[n] = make_uint2(v, at);
-                }
-              });
+            if (g0 + j * 32 < w1) {
+              const uint32_t g = g0 + j * 32, last = lo | 0x1FFFFFu;  // the bin's last key
+              auto in_bin = [&](uint32_t v) { return v >= lo && v <= last; };
+              auto note = [&](uint32_t v, uint32_t at) {
+                if (!in_bin(v)) return;
+                const uint32_t n = atomicAdd(&s_listed, 1u);
+                if (n < LIST) list[n] = make_uint2(v, at);
+              };
+              if (whole(g)) {  // few keys are in the bin: one branch for the group
+                sure += (k[j].x > last) + (k[j].y > last) + (k[j].z > last) + (k[j].w > last);
+                if (in_bin(k[j].x) || in_bin(k[j].y) || in_bin(k[j].z) || in_bin(k[j].w)) each(g, k[j], note);
+              } else {
+                each(g, k[j], [&](uint32_t v, uint32_t at) {
+                  sure += v > last;
+                  note(v, at);
+                });
+              }
+            }
         }
       }
       __syncthreads();

@@ -249,9 +249,12 @@ def _ptr(t):
 
 def _words(what, *tensors):
     """The kernels read and write 32-bit values: other widths (int64 lengths, half-precision queries) are refused."""
+    sizes = 4
     for t in tensors:
-        if t is not None and t.element_size() != 4:
-            raise ValueError(f"{what}: 32-bit tensors expected, got {t.dtype}")
+        if t is not None:
+            sizes |= t.itemsize
+    if sizes != 4:
+        raise ValueError(f"{what}: 32-bit tensors expected, got {[None if t is None else t.dtype for t in tensors]}")
 
 
 def _stream(s) -> C.c_void_p:
@@ -358,7 +361,8 @@ class DevicePool:
             raise ValueError("evict_select: keep [n_layers][n][>= budget], counts [n], contiguous positions")
         if (seq_ids.shape[0] if seq_ids is not None else lens.shape[0]) < n or (n > 1 and ms[1] != mass.shape[2]):
             raise ValueError(f"evict_select: {n} entries in mass, fewer sequences, or rows of mass apart")
-        _words("evict_select", mass, lens, keep, counts, seq_ids)
+        if (mass.itemsize | lens.itemsize | keep.itemsize | counts.itemsize) != 4 or seq_ids is not None:
+            _words("evict_select", mass, lens, keep, counts, seq_ids)
         rc = lib().kvcu_evict_select(self._h, nl, n, _ptr(seq_ids), lens.shape[0], lens.data_ptr(), budget, n_sink,
                                      n_recent, mass.data_ptr(), ms[0], mass.shape[2],
                                      keep.data_ptr(), kst[0], keep.shape[2] if n == 1 else kst[1], counts.data_ptr(),
