@@ -868,8 +868,10 @@ int kvcache_mla_attention_batch_lse_dev(kvcache* c, uint32_t layer, uint32_t seq
   if (!c || (n_pos && (!q_dev || !out_dev || !lse_dev))) return KVCU_ERR_INVALID_ARG;
   if (!n_pos) return KVCU_OK;
   DevScope d(c->device);
-  return attention_batch_impl(c, layer, seq, start_pos, n_pos, q_dev, n_heads, scale, out_dev, (cudaStream_t)stream,
-                              lse_dev);
+  return guarded("kvcache_mla_attention_batch_lse_dev", [&] {
+    return attention_batch_impl(c, layer, seq, start_pos, n_pos, q_dev, n_heads, scale, out_dev, (cudaStream_t)stream,
+                                lse_dev);
+  });
 }
 
 int kvcache_mla_attention_batch(kvcache* c, uint32_t layer, uint32_t seq, uint32_t start_pos, uint32_t n_pos,

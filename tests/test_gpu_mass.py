@@ -453,3 +453,39 @@ def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(kv, quant, 
     ws.test_withhold(0xFFFFFFFF)
     ws.set_wait_limit(0)
     assert torch.equal(run(), want) and cache.pool.status() == 0
+
+
+def test_many_columns_between_decodes_and_in_a_graph(kv):
+    """The decodes' partials lend their room: a decode after the sums gives the bits of one before, and
+    a captured window the bits of an eager one."""
+    import torch
+
+    cache = Paged(kv, [5000, 300, 64, 2049], 64, True, seed=15)
+    n_q, heads = 16, 20
+    q, lse = queries(cache, range(4), n_q, heads, 6)
+    ws = kv.DecodeWorkspace(0, 4, heads)
+    ws.plan(cache.pool, cache.lens_dev)
+    qd = q[:, 0].contiguous()
+    outs = [torch.empty(4, heads, 512, device="cuda") for _ in range(4)]
+    masses = [torch.zeros(4, 5000, device="cuda") for _ in range(4)]
+    decode = lambda o, **k: ws.decode(cache.pool, 0, qd, cache.toff, cache.tables, cache.lens_dev, SCALE, o, **k)
+    window = lambda m, **k: ws.attn_mass(cache.pool, 0, q, lse, cache.toff, cache.tables, cache.lens_dev, SCALE, m, **k)
+    decode(outs[0])
+    torch.cuda.synchronize()
+    for i in (1, 2):
+        window(masses[i])
+        decode(outs[i])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        s = torch.cuda.current_stream()
+        decode(outs[3], stream=s)
+        window(masses[3], stream=s)
+        decode(outs[3], stream=s)
+    for i in range(2):
+        masses[3].zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(masses[3], masses[1]) and torch.equal(outs[3], outs[0])
+    assert torch.equal(masses[1], masses[2]) and torch.equal(outs[1], outs[0]) and torch.equal(outs[2], outs[0])
+    assert cache.pool.status() == 0

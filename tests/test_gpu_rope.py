@@ -216,3 +216,20 @@ def test_refused_tensors(kv):
         r.apply(pos, x, q_out=x[:1].expand(4, 2, 64))
     r.apply(pos)  # nothing to rotate
     r.apply(pos[:0], x[:0])
+
+
+def test_positions_are_whole_numbers_and_may_be_one_of_many(kv):
+    import torch
+
+    rope = kv.Rope(64)
+    x = torch.randn(1, 3, 64, device="cuda")
+    with pytest.raises(ValueError):
+        rope.apply(torch.ones(1, device="cuda"), q=x)
+    with pytest.raises(ValueError):
+        rope.apply(torch.ones(1, dtype=torch.int64, device="cuda"), q=x)
+    many = torch.tensor([7, 8, 9, 10], dtype=torch.int32, device="cuda")
+    a, b = torch.empty_like(x), torch.empty_like(x)
+    rope.apply(many[1:2], q=x, q_out=a)
+    rope.apply(many[::4] + 1, q=x, q_out=b)  # a stride of its own, but one position
+    torch.cuda.synchronize()
+    assert torch.equal(a, b)
