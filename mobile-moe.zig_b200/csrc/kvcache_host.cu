@@ -528,7 +528,9 @@ int validate_positions(kvcache* c, uint32_t layer, uint32_t n, const uint32_t* s
 // prefix blocks stay read-only. The reference never writes into a shared
 // block, because only full blocks are cached and reusePrefixBlocks moves len past
 // them; this keeps that true after a truncate into a shared prefix as well.
-// Runs after validate_positions, on the stream of the write that follows.
+// Runs after validate_positions, on the stream of the write that follows, and after an
+// eviction on any stream: the blocks behind its budget are on the free list while its
+// moves still read them, and a block may hold rows that it has yet to move.
 int cow_for_write(kvcache* c, uint32_t n, const uint32_t* seq_ids, const uint32_t* positions,
                   cudaStream_t st) {
   for (uint32_t r = 0; r < n; ++r) {
@@ -539,7 +541,8 @@ int cow_for_write(kvcache* c, uint32_t n, const uint32_t* seq_ids, const uint32_
     uint32_t fresh;
     int rc = allocate_block(c, &fresh);
     if (rc) return rc;
-    rc = kvcu_pool_copy_block(c->pool, old, fresh, st);
+    rc = after_eviction(c, st);
+    if (!rc) rc = kvcu_pool_copy_block(c->pool, old, fresh, st);
     if (rc) {
       release_block(c, fresh);
       return rc;
