@@ -663,8 +663,8 @@ int kvcache_attn_mass_dev(kvcache* c, uint32_t layer, uint32_t n, const uint32_t
  * rows are no longer those of consecutive tokens).  keep_dev (device, may be NULL)
  * receives the kept positions [n_layers][n][budget].  Call it between steps,
  * when every layer holds the sequences' rows, ordered after the calls that
- * wrote or read them; the cache's next append, step, decode or gather, on any
- * stream, runs after it. */
+ * wrote or read them; the cache's next append, step, decode, gather, save or
+ * load, on any stream, runs after it. */
 int kvcache_evict_dev(kvcache* c, uint32_t n, const uint32_t* seq_ids, uint32_t budget, uint32_t n_sink,
                       uint32_t n_recent, float* mass_dev, uint64_t mass_layer_stride, uint64_t mass_stride,
                       uint32_t* keep_dev, void* stream);

@@ -921,7 +921,10 @@ void kvcache_deinit(kvcache* c) {
   if (c->save_stg) cudaFree(c->save_stg);
   for (uint8_t* h : c->save_host)
     if (h) cudaFreeHost(h);
-  if (c->stream) cudaStreamSynchronize(c->stream);
+  if (c->stream) {
+    after_eviction(c, c->stream);
+    cudaStreamSynchronize(c->stream);
+  }
   kvcu_decode_ws_destroy(c->ws);
   kvcu_pool_destroy(c->pool);
   cudaFree(c->d_toff);
@@ -958,6 +961,7 @@ int kvcache_enable_quantization(kvcache* c) {
   kvcu_pool* q = kvcu_pool_create(c->device, c->n_layers, c->num_blocks, c->block_size, c->kv_rank,
                                   c->rope_dim, 1);
   if (!q) return KVCU_ERR_NO_MEMORY;
+  after_eviction(c, c->stream);
   cudaStreamSynchronize(c->stream);
   kvcu_pool_destroy(c->pool);
   c->pool = q;
@@ -1542,6 +1546,7 @@ struct IoBuffers {
 int write_pool(kvcache* c, int fd) {
   kvcu_pool_desc desc;
   int rc = kvcu_pool_describe(c->pool, &desc);
+  if (!rc) rc = after_eviction(c, c->stream);  // the lengths and tables written are those behind it
   if (rc) return rc;
   const uint64_t total = desc.checkpoint_bytes;
   const size_t chunk = (size_t)std::min<uint64_t>(kIoChunk, std::max<uint64_t>(total, 1));
@@ -1567,6 +1572,7 @@ int write_pool(kvcache* c, int fd) {
 int read_pool(kvcache* c, int fd) {
   kvcu_pool_desc desc;
   int rc = kvcu_pool_describe(c->pool, &desc);
+  if (!rc) rc = after_eviction(c, c->stream);  // whose moves would land in the rows read here
   if (rc) return rc;
   const uint64_t total = desc.checkpoint_bytes;
   if (!total) return KVCU_OK;
@@ -1918,7 +1924,9 @@ int kvcache_save_to_file_v2_async(kvcache* c, const char* path, void* stream, kv
   if (!c->save_stg) KVCU_CUDA(cudaMalloc(&c->save_stg, kSaveChunk));
   for (auto& h : c->save_host)
     if (!h) KVCU_CUDA(cudaHostAlloc(reinterpret_cast<void**>(&h), kSaveChunk, cudaHostAllocDefault));
-  // start after the caller's stream and the cache's own stream
+  // start after the caller's stream, the cache's own stream and an eviction on any
+  const int rc = after_eviction(c, c->stream);
+  if (rc) return rc;
   cudaEvent_t start = nullptr;
   KVCU_CUDA(cudaEventCreateWithFlags(&start, cudaEventDisableTiming));
   if (stream) {

@@ -23,7 +23,7 @@ class Evicted:
     blocks behind the budget, which the host has given back already.  Sequence 1 holds 70 rows,
     the first 64 of them shared with sequence 2."""
 
-    def __init__(self, kv, quant):
+    def __init__(self, kv, quant, before=lambda cache: None):
         import torch
 
         self.c = c = make(kv, [1280, 70, 0], quant, LAYERS, spare=2)
@@ -35,6 +35,7 @@ class Evicted:
             prefix = kv.KVCache.computeHash(part, prefix)
         c.seq_reuse_prefix_blocks(2, self.tokens, 4)
         self.rows = [[c.gather(layer, s) for s in range(3)] for layer in range(LAYERS)]
+        before(c)
         self.mass = torch.arange(1280, device="cuda", dtype=torch.float32).repeat(LAYERS, 1, 1)
         self.keep = torch.empty(LAYERS, 1, 640, dtype=torch.int32, device="cuda")
         # once within the budget, which changes nothing: kernels loaded and scratch there, so that the host does not wait
@@ -118,3 +119,33 @@ def test_host_appends_and_steps_after_an_eviction(kv):
     for layer in range(LAYERS):
         st.run(c, layer, [2], [60], kv.Rope(P), stream=f.other)
     f.check(lambda layer: np.concatenate([f.rows[layer][2][:60], c.gather(layer, 2)[60:]]))
+
+
+@pytest.mark.parametrize("how", ["v1", "v2", "background"])
+def test_a_save_after_an_eviction_holds_its_rows(kv, tmp_path, how):
+    e = Evicted(kv, True)
+    at = tmp_path / "save.ckpt"
+    if how == "v1":  # sequence 0 alone
+        e.c.saveToFile(at)
+    elif how == "v2":
+        e.c.saveToFileV2(at)
+    else:
+        e.c.saveToFileV2Async(at).wait()
+    e.check(lambda layer: e.rows[layer][2])
+    d = kv.KVCache.with_blocks(LAYERS, 512, P, e.c.num_blocks, BS, quantized=True)
+    if how == "v1":
+        d.loadFromFile(at)
+    else:
+        d.loadFromFileV2(at)
+    for layer in range(LAYERS):
+        assert np.array_equal(d.gather(layer, 0), e.rows[layer][0][640:])
+        for s in (1, 2) if how != "v1" else ():
+            assert np.array_equal(d.gather(layer, s), e.rows[layer][s])
+
+
+def test_a_load_after_an_eviction_keeps_what_it_read(kv, tmp_path):
+    e = Evicted(kv, True, before=lambda cache: cache.saveToFileV2(tmp_path / "save.ckpt"))
+    e.c.loadFromFileV2(tmp_path / "save.ckpt")
+    for layer in range(LAYERS):
+        for s in range(3):
+            assert np.array_equal(e.c.gather(layer, s), e.rows[layer][s])
