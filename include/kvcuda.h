@@ -658,7 +658,7 @@ int kvcache_attn_mass_dev(kvcache* c, uint32_t layer, uint32_t n, const uint32_t
  * mass [n_layers][n][mass_stride] moved along; its length becomes budget and the
  * blocks behind return to the pool, as after a truncate.  Blocks held elsewhere
  * (a shared prefix, a running save) are copied before rows move into them
- * (KVCU_ERR_OUT_OF_BLOCKS where none is free; nothing is evicted then), and
+ * (KVCU_ERR_OUT_OF_BLOCKS where too few are free; nothing has changed then), and
  * rewritten blocks leave the prefix cache (and must not be entered again: their
  * rows are no longer those of consecutive tokens).  keep_dev (device, may be NULL)
  * receives the kept positions [n_layers][n][budget].  Call it between steps,

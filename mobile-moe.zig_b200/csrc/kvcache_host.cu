@@ -1451,27 +1451,39 @@ int kvcache_evict_dev(kvcache* c, uint32_t n, const uint32_t* seq_ids, uint32_t 
       any = any || c->seqs[s].len > budget;
     }
     if (!any && !keep_dev) return KVCU_OK;
-    // The blocks that rows move into: copied first where another sequence or a
-    // running save holds them too, and no longer what their prefix hash says.
+    // f(sequence, block index) over the blocks that rows move into, until it fails.
     // Blocks wholly inside the first n_sink positions keep their rows.
-    for (uint32_t b = 0; b < n; ++b) {
-      Seq& q = c->seqs[seq_ids[b]];
-      if (q.len <= budget) continue;
-      const uint32_t end = (uint32_t)(((uint64_t)budget + c->block_size - 1) / c->block_size);
-      for (uint32_t bi = n_sink / c->block_size; bi < end; ++bi) {
-        const uint32_t pos = bi * c->block_size;
-        const int rc = cow_for_write(c, 1, seq_ids + b, &pos, st);
-        if (rc) return rc;
-        const uint32_t id = q.table[bi];
-        if (c->hash[id] != kNoHash) {
-          auto it = c->hash_map.find(c->hash[id]);
-          if (it != c->hash_map.end() && it->second == id) c->hash_map.erase(it);
-          c->hash[id] = kNoHash;
+    const uint32_t end = (uint32_t)(((uint64_t)budget + c->block_size - 1) / c->block_size);
+    auto rewritten = [&](auto&& f) -> int {
+      for (uint32_t b = 0; b < n; ++b)
+        for (uint32_t bi = n_sink / c->block_size; c->seqs[seq_ids[b]].len > budget && bi < end; ++bi) {
+          const int rc = f(seq_ids[b], bi);
+          if (rc) return rc;
         }
-      }
+      return KVCU_OK;
+    };
+    // Those that another sequence or a running save holds too are copied first.  The
+    // copies are counted before any is made, as a copy leaves one holder less to the next.
+    std::unordered_map<uint32_t, uint32_t> holders;
+    size_t copies = 0;
+    rewritten([&](uint32_t s, uint32_t bi) -> int {
+      const uint32_t id = c->seqs[s].table[bi];
+      if (c->ref_count[id] <= 1) return KVCU_OK;
+      uint32_t& left = holders.emplace(id, c->ref_count[id]).first->second;
+      if (left > 1) --left, ++copies;
+      return KVCU_OK;
+    });
+    if (copies > c->free_list.size()) {
+      kvcu_set_error("OutOfKVCacheBlocks: %zu shared blocks to copy, %zu free", copies, c->free_list.size());
+      return KVCU_ERR_OUT_OF_BLOCKS;
     }
     const size_t list = keep_dev ? 0 : (size_t)c->n_layers * n * budget;
     int rc = bound_acquire(c, 2 * (size_t)n + list, n, st);
+    if (!rc)
+      rc = rewritten([&](uint32_t s, uint32_t bi) -> int {
+        const uint32_t pos = bi * c->block_size;
+        return cow_for_write(c, 1, &s, &pos, st);
+      });
     if (!rc) rc = sync_tables(c, st);
     if (!rc) rc = sync_lens(c, st);
     if (rc) return rc;
@@ -1490,6 +1502,16 @@ int kvcache_evict_dev(kvcache* c, uint32_t n, const uint32_t* seq_ids, uint32_t 
                               st);
     KVCU_CUDA(cudaEventRecord(c->bound_done, st));
     if (rc) return rc;
+    // the rewritten blocks are no longer what their prefix hash says
+    rewritten([&](uint32_t s, uint32_t bi) -> int {
+      const uint32_t id = c->seqs[s].table[bi];
+      if (c->hash[id] != kNoHash) {
+        auto it = c->hash_map.find(c->hash[id]);
+        if (it != c->hash_map.end() && it->second == id) c->hash_map.erase(it);
+        c->hash[id] = kNoHash;
+      }
+      return KVCU_OK;
+    });
     for (uint32_t b = 0; b < n; ++b)
       if (c->seqs[seq_ids[b]].len > budget) seq_truncate(c, seq_ids[b], budget);
     if (any) c->tables_dirty = c->lens_dirty = true;  // the next upload, on any stream, waits for the moves
