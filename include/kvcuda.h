@@ -396,12 +396,14 @@ int kvcu_evict_select(kvcu_pool* pool, uint32_t n_layers, uint32_t n, const uint
 /* Row j of entry b's sequence := its row keep[..][j], j < keep_counts[b], in
  * layers [layer, layer + n_layers) (keep's layer i for layer + i), in place
  * through the block table; mass (may be NULL) moves along, mass[j] :=
- * mass[keep[j]]; lens (may be NULL): lens[seq] := keep_counts[b].  keep must
- * ascend strictly, and a sequence may appear once in the batch.  Rows behind
- * the kept ones are left as they were (free them by truncating the table);
- * blocks are written whoever else holds them, so shared blocks must be copied
- * first (kvcu_pool_copy_block).  Entries that point
- * outside the table or the pool set the status word and their row is left. */
+ * mass[keep[j]] (strides as for kvcu_evict_select; rows that overlap are refused,
+ * a position beyond its row sets KVCU_STATUS_BAD_LEN and its sum becomes 0);
+ * lens (may be NULL): lens[seq] := keep_counts[b].  keep must ascend strictly,
+ * and a sequence may appear once in the batch.  Rows behind the kept ones are
+ * left as they were (free them by truncating the table); blocks are written
+ * whoever else holds them, so shared blocks must be copied first
+ * (kvcu_pool_copy_block).  Entries that point outside the table or the pool set
+ * the status word and their row is left. */
 int kvcu_evict_compact(kvcu_pool* pool, uint32_t layer, uint32_t n_layers, uint32_t n, const uint32_t* seq_ids,
                        uint32_t n_seqs, const uint32_t* table_offsets, const uint32_t* tables, const uint32_t* keep,
                        uint64_t keep_layer_stride, uint64_t keep_stride, const uint32_t* keep_counts, float* mass,
@@ -655,9 +657,9 @@ int kvcache_attn_mass_dev(kvcache* c, uint32_t layer, uint32_t n, const uint32_t
 /* Bring every listed sequence (each once) that is longer than `budget` down to
  * budget rows in all layers: per layer the first n_sink, the last n_recent and
  * the rows of the largest mass between (kvcu_evict_select, kvcu_evict_compact),
- * mass [n_layers][n][mass_stride] moved along; its length becomes budget and the
- * blocks behind return to the pool, as after a truncate.  Blocks held elsewhere
- * (a shared prefix, a running save) are copied before rows move into them
+ * mass [n_layers][n][mass_stride] moved along (rows that overlap are refused);
+ * its length becomes budget and the blocks behind return to the pool, as after
+ * a truncate.  Blocks held elsewhere (a shared prefix, a running save) are copied before rows move into them
  * (KVCU_ERR_OUT_OF_BLOCKS where too few are free; nothing has changed then), and
  * rewritten blocks leave the prefix cache (and must not be entered again: their
  * rows are no longer those of consecutive tokens).  keep_dev (device, may be NULL)

@@ -1434,6 +1434,12 @@ int kvcache_evict_dev(kvcache* c, uint32_t n, const uint32_t* seq_ids, uint32_t 
   DevScope d(c->device);
   const cudaStream_t st = (cudaStream_t)stream;
   return guarded("kvcache_evict_dev", [&]() -> int {
+    const uint64_t mass_row = kvcu_mass_row(c->n_layers, n, mass_layer_stride, mass_stride);
+    if (!mass_row) {
+      kvcu_set_error("kvcache_evict_dev: rows of sums overlap at strides %llu (layers) and %llu (sequences)",
+                     (unsigned long long)mass_layer_stride, (unsigned long long)mass_stride);
+      return KVCU_ERR_INVALID_ARG;
+    }
     std::vector<char> seen(c->seqs.size(), 0);
     bool any = false;
     for (uint32_t b = 0; b < n; ++b) {
@@ -1443,9 +1449,9 @@ int kvcache_evict_dev(kvcache* c, uint32_t n, const uint32_t* seq_ids, uint32_t 
         return KVCU_ERR_INVALID_ARG;
       }
       seen[s] = 1;
-      if (c->seqs[s].len > mass_stride) {
+      if (c->seqs[s].len > mass_row) {
         kvcu_set_error("kvcache_evict_dev: sequence %u holds %u positions, a row of sums %llu", s, c->seqs[s].len,
-                       (unsigned long long)mass_stride);
+                       (unsigned long long)mass_row);
         return KVCU_ERR_INVALID_ARG;
       }
       any = any || c->seqs[s].len > budget;

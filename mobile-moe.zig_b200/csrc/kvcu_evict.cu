@@ -374,7 +374,7 @@ struct CompactArgs {
   uint64_t keep_lstride, keep_stride;
   const uint32_t* counts;
   float* mass;
-  uint64_t mass_lstride, mass_stride;
+  uint64_t mass_lstride, mass_stride, mass_row;  // mass_row: positions of a row of sums
   uint32_t* lens;
   uint32_t* status;
   uint32_t tile;  // rows of a CTA's tile
@@ -456,7 +456,10 @@ __global__ void __launch_bounds__(CT) k_evict_compact(CompactArgs a, uint32_t C)
     }
     blk_src = a.tables[t0 + at / a.block_size];
     blk_dst = a.tables[t0 + j / a.block_size];
-    if (mass) val = at < a.mass_stride ? __ldcg(mass + at) : 0.0f;
+    if (!mass) return;
+    val = 0.0f;
+    if (at < a.mass_row) val = __ldcg(mass + at);
+    else atomicOr(a.status, KVCU_STATUS_BAD_LEN);
   };
   auto load = [&](uint32_t w) {  // the copies of wave w, resolved before
     const uint32_t f = w & 1u;
@@ -513,7 +516,7 @@ __global__ void __launch_bounds__(CT) k_evict_compact(CompactArgs a, uint32_t C)
     }
     if (mass && tid < a.tile && src_row[f][tid] != NO_ROW) {
       const uint32_t j = (w * C + rank) * a.tile + tid;
-      if (j < a.mass_stride) mass[j] = mval[f][tid];
+      if (j < a.mass_row) mass[j] = mval[f][tid];
     }
     __syncthreads();  // the stage may be filled again
   }
@@ -612,7 +615,10 @@ __global__ void __launch_bounds__(CT, 3) k_evict_compact_wide(CompactArgs a, uin
     }
     blk_src = a.tables[t0 + at / a.block_size];
     blk_dst = a.tables[t0 + j / a.block_size];
-    if (mass) val_next = at < a.mass_stride ? __ldcg(mass + at) : 0.0f;
+    if (!mass) return;
+    val_next = 0.0f;
+    if (at < a.mass_row) val_next = __ldcg(mass + at);
+    else atomicOr(a.status, KVCU_STATUS_BAD_LEN);
   };
   auto publish = [&](uint32_t w, float& v) {
     if (tid >= a.tile) return;
@@ -656,7 +662,7 @@ __global__ void __launch_bounds__(CT, 3) k_evict_compact_wide(CompactArgs a, uin
       const uint64_t r = dst_row[w & 1u][row_in(word[i])];
       if (r != NO_ROW) *word_at(word[i], r) = v.word[i];
     }
-    if (mass && tid < a.tile && dst_row[w & 1u][tid] != NO_ROW && row_j(w) < a.mass_stride) mass[row_j(w)] = m;
+    if (mass && tid < a.tile && dst_row[w & 1u][tid] != NO_ROW && row_j(w) < a.mass_row) mass[row_j(w)] = m;
   };
   Wave even, odd;
   fetch(0);
@@ -778,6 +784,17 @@ extern "C" int kvcu_evict_select(kvcu_pool* pool, uint32_t n_layers, uint32_t n,
   return launch_select<8>(a, (uint32_t)rows, st);
 }
 
+uint64_t kvcu_mass_row(uint32_t n_layers, uint32_t n, uint64_t layer_stride, uint64_t stride) {
+  if (n_layers <= 1) return stride;
+  const uint64_t small = layer_stride < stride ? layer_stride : stride, large = layer_stride < stride ? stride : layer_stride;
+  if (n <= 1) return small;
+  // the rows of the smaller stride lie between two of the larger
+  const uint64_t steps = (layer_stride < stride ? n_layers : n) - 1u;
+  if (small == 0 || large / steps < small || large == steps * small) return 0;
+  const uint64_t last = large - steps * small;
+  return small < last ? small : last;
+}
+
 extern "C" int kvcu_evict_compact(kvcu_pool* pool, uint32_t layer, uint32_t n_layers, uint32_t n, const uint32_t* seq_ids,
                                   uint32_t n_seqs, const uint32_t* table_offsets, const uint32_t* tables,
                                   const uint32_t* keep, uint64_t keep_layer_stride, uint64_t keep_stride,
@@ -798,6 +815,12 @@ extern "C" int kvcu_evict_compact(kvcu_pool* pool, uint32_t layer, uint32_t n_la
   if (pairs > 0x7FFFFFFu || !keep_stride) {
     kvcu_set_error("kvcu_evict_compact: %llu (layer, entry) pairs, keep stride %llu", (unsigned long long)pairs,
                    (unsigned long long)keep_stride);
+    return KVCU_ERR_INVALID_ARG;
+  }
+  const uint64_t mass_row = mass ? kvcu_mass_row(n_layers, n, mass_layer_stride, mass_stride) : 0;
+  if (mass && !mass_row) {
+    kvcu_set_error("kvcu_evict_compact: rows of sums overlap at strides %llu (layers) and %llu (entries)",
+                   (unsigned long long)mass_layer_stride, (unsigned long long)mass_stride);
     return KVCU_ERR_INVALID_ARG;
   }
   DevScope d(pool->device);
@@ -830,6 +853,7 @@ extern "C" int kvcu_evict_compact(kvcu_pool* pool, uint32_t layer, uint32_t n_la
   a.mass = mass;
   a.mass_lstride = mass_layer_stride;
   a.mass_stride = mass_stride;
+  a.mass_row = mass_row;
   a.lens = lens;
   a.status = pool->status;
   const uint64_t sms = (uint64_t)kvcu_current_sm_count();

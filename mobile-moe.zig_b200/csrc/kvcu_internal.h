@@ -115,6 +115,9 @@ int kvcu_current_sm_count();
 // Dynamic shared memory the eviction kernels may ask for (184 KB: 46k keys of a
 // row; their static arrays take up to 33 KB more of an SM's 227 KB).
 #define KVCU_EVICT_SMEM 188416
+// Positions that each of the n_layers x n rows of sums at these strides has to itself
+// (0: some overlap); an eviction moves the sums of all rows in place at once.
+uint64_t kvcu_mass_row(uint32_t n_layers, uint32_t n, uint64_t layer_stride, uint64_t stride);
 
 // ---- kernel launchers (kvcu_kernels.cu) ----
 int kvcu_launch_append(kvcu_pool* p, uint32_t layer, uint32_t n_rows, const float* latent,

@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 
+from pooldata import Paged, arrays
 from test_gpu_bounded import BS, kv, make  # noqa: F401 (kv is the module's fixture)
 from test_gpu_evict import want_keep
 
@@ -62,3 +63,65 @@ def test_just_enough_blocks_for_the_copies(kv, ids):
     assert c.findPrefixBlocks(t) == (0 if len(ids) == 2 else 6)
     live = {b for s in range(2) for b in c.seq_block_table(s)}
     assert c.numFreeBlocks() + len(live) == c.num_blocks
+
+
+def compact(kv, cache, keep, counts, mass, layer_stride, stride):
+    """The C call, with any strides of the sums."""
+    layers, n, budget = keep.shape
+    return kv.lib().kvcu_evict_compact(cache.pool.handle, 0, layers, n, None, n, cache.toff.data_ptr(),
+                                       cache.tables.data_ptr(), keep.data_ptr(), n * budget, budget, counts.data_ptr(),
+                                       mass.data_ptr(), layer_stride, stride, None, None)
+
+
+def test_rows_of_sums_that_overlap(kv):
+    """All rows of sums move at once, so no two may share one."""
+    import torch
+
+    cache = Paged(kv, [200, 200, 200], 16, True, layers=2, seed=4)
+    before = [x.clone() for x in arrays(cache.pool)]
+    keep = torch.arange(100, dtype=torch.int32, device="cuda").mul_(2).repeat(2, 3, 1)
+    counts = torch.full((3,), 100, dtype=torch.int32, device="cuda")
+    mass = torch.rand(2, 3, 200, device="cuda")
+    kept = mass.clone()
+    # no layers apart, no entries apart, no row between, layers inside the entries, entries inside the layers
+    for strides in ((0, 200), (600, 0), (0, 0), (200, 200), (400, 200), (200, 100), (2 ** 63, 2 ** 63)):
+        assert compact(kv, cache, keep, counts, mass, *strides) == -11, strides
+    with pytest.raises(kv.KVCudaError):
+        cache.pool.evict_compact(0, cache.toff, cache.tables, keep, counts, mass=mass[:1].expand(2, 3, 200))
+    c, _ = shared(kv, 8)
+    for strides in ((0, 96), (96, 96), (96, 0)):
+        ids = np.array([0, 1], np.uint32)
+        assert kv.lib().kvcache_evict_dev(c._h, 2, ids.ctypes.data, 64, 0, 0, mass.data_ptr(), *strides, None, None) == -11
+    assert c.seq_len(0) == 96 and c.numFreeBlocks() == 8
+    torch.cuda.synchronize()
+    assert torch.equal(mass, kept) and all(torch.equal(a, b) for a, b in zip(arrays(cache.pool), before))
+
+
+def test_sums_with_the_layers_inside_the_entries(kv):
+    """[entry][layer][position] is a layout of its own, and one entry's rows may be any distance apart."""
+    import torch
+
+    for n in (3, 1):
+        cache = Paged(kv, [200] * n, 16, True, layers=2, seed=4)
+        keep = torch.arange(100, dtype=torch.int32, device="cuda").mul_(2).repeat(2, n, 1)
+        counts = torch.full((n,), 100, dtype=torch.int32, device="cuda")
+        mass = torch.rand(n, 2, 200, device="cuda")
+        want = mass.clone()
+        want[:, :, :100] = mass[:, :, :200:2]
+        assert compact(kv, cache, keep, counts, mass, 200, 400) == 0
+        assert cache.pool.status() == 0 and torch.equal(mass, want)
+
+
+@pytest.mark.parametrize("dims", [(512, 64), (64, 32)])  # rows moved through registers, and through shared memory
+def test_a_kept_position_beyond_its_row_of_sums(kv, dims):
+    import torch
+
+    cache = Paged(kv, [200], 16, True, layers=2, seed=4, dims=dims)
+    keep = torch.arange(100, dtype=torch.int32, device="cuda").mul_(2).repeat(2, 1, 1)
+    counts = torch.full((1,), 100, dtype=torch.int32, device="cuda")
+    mass = torch.rand(2, 1, 150, device="cuda") + 1
+    want = mass.clone()
+    want[:, :, :75] = mass[:, :, ::2]
+    want[:, :, 75:100] = 0
+    cache.pool.evict_compact(0, cache.toff, cache.tables, keep, counts, mass=mass)
+    assert cache.pool.status() == 0x8 and torch.equal(mass, want)
