@@ -247,14 +247,41 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _words(what, *tensors):
-    """The kernels read and write 32-bit values: other widths (int64 lengths, half-precision queries) are refused."""
-    sizes = 4
+_types = ()
+
+
+def _dtypes():
+    """float32, and the types of lengths, tables and positions."""
+    global _types
+    if not _types:
+        import torch
+
+        _types = torch.float32, (torch.int32, torch.uint32)
+    return _types
+
+
+def _reals(what, device, *tensors):
+    """f32 tensors of the device (or None): the kernels get plain addresses, so nothing else may pass."""
+    f32 = _dtypes()[0]
     for t in tensors:
-        if t is not None:
-            sizes |= t.itemsize
-    if sizes != 4:
-        raise ValueError(f"{what}: 32-bit tensors expected, got {[None if t is None else t.dtype for t in tensors]}")
+        if t is not None and (t.dtype is not f32 or t.get_device() != device):
+            raise ValueError(f"{what}: float32 tensors on cuda:{device} expected, got {t.dtype} on {t.device}")
+
+
+def _whole(what, device, *tensors):
+    """Contiguous 32-bit whole numbers on the device (or None): lengths, block tables, ids, counts."""
+    kinds = _dtypes()[1]
+    for t in tensors:
+        if t is not None and (t.dtype not in kinds or t.get_device() != device or not t.is_contiguous()):
+            raise ValueError(f"{what}: contiguous 32-bit integer tensors on cuda:{device} expected, got {t.dtype} on "
+                             f"{t.device} with strides {tuple(t.stride())}")
+
+
+def _holds(what, t, words):
+    """A contiguous tensor (or None) of at least `words` elements."""
+    if t is not None and (t.numel() < words or not t.is_contiguous()):
+        raise ValueError(f"{what}: a contiguous tensor of {words} elements expected, got {tuple(t.shape)} with strides "
+                         f"{tuple(t.stride())}")
 
 
 def _stream(s) -> C.c_void_p:
@@ -361,8 +388,10 @@ class DevicePool:
             raise ValueError("evict_select: keep [n_layers][n][>= budget], counts [n], contiguous positions")
         if (seq_ids.shape[0] if seq_ids is not None else lens.shape[0]) < n or (n > 1 and ms[1] != mass.shape[2]):
             raise ValueError(f"evict_select: {n} entries in mass, fewer sequences, or rows of mass apart")
-        if (mass.itemsize | lens.itemsize | keep.itemsize | counts.itemsize) != 4 or seq_ids is not None:
-            _words("evict_select", mass, lens, keep, counts, seq_ids)
+        _reals("evict_select", self.device, mass)
+        _whole("evict_select", self.device, lens, counts, seq_ids)
+        if keep.dtype not in _types[1] or keep.get_device() != self.device:
+            raise ValueError(f"evict_select: keep of 32-bit integers on cuda:{self.device} expected, got {keep.dtype}")
         rc = lib().kvcu_evict_select(self._h, nl, n, _ptr(seq_ids), lens.shape[0], lens.data_ptr(), budget, n_sink,
                                      n_recent, mass.data_ptr(), ms[0], mass.shape[2],
                                      keep.data_ptr(), kst[0], keep.shape[2] if n == 1 else kst[1], counts.data_ptr(),
@@ -383,7 +412,12 @@ class DevicePool:
         n_seqs = table_offsets.shape[0] - 1
         if (seq_ids.shape[0] if seq_ids is not None else n_seqs) < n or counts.shape[0] < n:
             raise ValueError(f"evict_compact: {n} entries in keep, fewer sequences or counts")
-        _words("evict_compact", table_offsets, tables, keep, counts, mass, lens, seq_ids)
+        if lens is not None and lens.shape[0] < n_seqs:
+            raise ValueError(f"evict_compact: tables of {n_seqs} sequences, lens of {lens.shape[0]}")
+        _reals("evict_compact", self.device, mass)
+        _whole("evict_compact", self.device, table_offsets, tables, counts, lens, seq_ids)
+        if keep.dtype not in _types[1] or keep.get_device() != self.device:
+            raise ValueError(f"evict_compact: keep of 32-bit integers on cuda:{self.device} expected, got {keep.dtype}")
         ms = (0, 0) if mass is None else (mass.stride(0), mass.shape[2])
         rc = lib().kvcu_evict_compact(self._h, layer, nl, n, _ptr(seq_ids), n_seqs, table_offsets.data_ptr(),
                                       tables.data_ptr(), keep.data_ptr(), kst[0], keep.shape[2], counts.data_ptr(), _ptr(mass),
@@ -448,14 +482,16 @@ class DecodeWorkspace:
         log-sum-exp lse [n][n_q][H], on the last plan (kvcu_attn_mass)."""
         n, H, W = q.shape[0], q.shape[-2], q.shape[-1]
         n_q = q.shape[1] if q.dim() == 4 else 1
-        if not (q.is_contiguous() and lse.is_contiguous()) or lse.numel() != n * n_q * H or mass.stride(-1) != 1:
+        if not (q.is_contiguous() and lse.is_contiguous()) or lse.numel() != n * n_q * H or mass.dim() != 2 or (
+                mass.stride(1) != 1):
             raise ValueError("attn_mass: contiguous q [n][n_q][H][W] and lse [n][n_q][H], mass [n][positions]")
         if mass.shape[0] != n or (n > 1 and mass.stride(0) != mass.shape[1]) or table_offsets.shape[0] <= lens.shape[0] or (
                 old_lens is not None and old_lens.shape[0] < n):
             raise ValueError(f"attn_mass: {n} entries in q, other sizes in mass, old_lens or table_offsets")
         if W != 576 or (seq_ids is not None and seq_ids.shape[0] < n):  # the kernels' row width
             raise ValueError(f"attn_mass: queries of {W} elements, 576 expected, or fewer seq_ids than entries")
-        _words("attn_mass", q, lse, table_offsets, tables, lens, mass, old_lens, seq_ids)
+        _reals("attn_mass", pool.device, q, lse, mass)
+        _whole("attn_mass", pool.device, table_offsets, tables, lens, old_lens, seq_ids)
         rc = lib().kvcu_attn_mass(self._h, pool.handle, layer, n, _ptr(seq_ids), lens.shape[0], table_offsets.data_ptr(),
                                   tables.data_ptr(), lens.data_ptr(), n_q, q.data_ptr(), lse.data_ptr(), H, scale, decay,
                                   _ptr(old_lens), mass.data_ptr(), mass.shape[1], _stream(stream))
@@ -914,10 +950,11 @@ class KVCache:
         n, H = q.shape[0], q.shape[1]
         if s.size != n or p.size != n or (rp is not None and rp.size != n):
             raise ValueError(f"mla_step_rope_dev: {n} queries, other numbers of sequences or positions")
-        _words("mla_step_rope_dev", q, kv_a, norm_w, k_b, v_b, attn, q_abs, lse)
-        if ((q_abs is not None and (q_abs.numel() < n * H * (self.kv_rank + self.rope_dim) or not q_abs.is_contiguous()))
-                or (lse is not None and (lse.numel() < n * H or not lse.is_contiguous()))):
-            raise ValueError(f"mla_step_rope_dev: q_abs [{n}][{H}][{self.kv_rank + self.rope_dim}], lse [{n}][{H}]")
+        R, W = self.kv_rank, self.kv_rank + self.rope_dim
+        _reals("mla_step_rope_dev", self.device, q, kv_a, norm_w, k_b, v_b, attn, q_abs, lse)
+        for t, words in ((q, n * H * (qk_nope + self.rope_dim)), (kv_a, n * W), (norm_w, R), (k_b, H * qk_nope * R),
+                         (v_b, H * v_dim * R), (attn, n * H * v_dim), (q_abs, n * H * W), (lse, n * H)):
+            _holds("mla_step_rope_dev", t, words)
         check(lib().kvcache_mla_step_rope_dev(self._h, layer, n, _np_ptr(s), _np_ptr(p), rope.handle,
                                               None if rp is None else _np_ptr(rp), _dptr(q), _dptr(kv_a),
                                               _dptr(norm_w), eps, _dptr(k_b), _dptr(v_b), H, qk_nope, v_dim, scale,
@@ -928,18 +965,22 @@ class KVCache:
         """mlaDecode_dev that also writes lse [n][H], the log-sum-exp of the scaled scores."""
         s = np.ascontiguousarray(seq_ids, np.uint32)
         n, H = q_dev.shape[0], q_dev.shape[1]
-        _words("mlaDecodeLse_dev", q_dev, out_dev, lse_dev)
-        if q_dev.shape[2] != self.kv_rank + self.rope_dim or lse_dev.numel() < n * H:
-            raise ValueError(f"mlaDecodeLse_dev: q [{n}][{H}][{self.kv_rank + self.rope_dim}], lse [{n}][{H}]")
+        if s.size != n or q_dev.shape[2] != self.kv_rank + self.rope_dim:
+            raise ValueError(f"mlaDecodeLse_dev: {s.size} sequences, q [n][H][{self.kv_rank + self.rope_dim}] expected")
+        _reals("mlaDecodeLse_dev", self.device, q_dev, out_dev, lse_dev)
+        for t, words in ((q_dev, 0), (out_dev, n * H * self.kv_rank), (lse_dev, n * H)):
+            _holds("mlaDecodeLse_dev", t, words)
         check(lib().kvcache_mla_decode_lse_dev(self._h, layer, n, _np_ptr(s), _dptr(q_dev), H, scale, _dptr(out_dev),
                                                _dptr(lse_dev), _stream(stream)), "mlaDecodeLse_dev")
 
     def mlaAttentionBatchLse_dev(self, layer, seq, start_pos, q_dev, scale, out_dev, lse_dev, stream=None):
         """mlaAttentionBatch_dev that also writes lse [n_pos][H]."""
         n, H = q_dev.shape[0], q_dev.shape[1]
-        _words("mlaAttentionBatchLse_dev", q_dev, out_dev, lse_dev)
-        if q_dev.shape[2] != self.kv_rank + self.rope_dim or lse_dev.numel() < n * H:
-            raise ValueError(f"mlaAttentionBatchLse_dev: q [{n}][{H}][{self.kv_rank + self.rope_dim}], lse [{n}][{H}]")
+        if q_dev.shape[2] != self.kv_rank + self.rope_dim:
+            raise ValueError(f"mlaAttentionBatchLse_dev: q [n_pos][H][{self.kv_rank + self.rope_dim}] expected")
+        _reals("mlaAttentionBatchLse_dev", self.device, q_dev, out_dev, lse_dev)
+        for t, words in ((q_dev, 0), (out_dev, n * H * self.kv_rank), (lse_dev, n * H)):
+            _holds("mlaAttentionBatchLse_dev", t, words)
         check(lib().kvcache_mla_attention_batch_lse_dev(self._h, layer, seq, start_pos, n, _dptr(q_dev), H, scale,
                                                         _dptr(out_dev), _dptr(lse_dev), _stream(stream)),
               "mlaAttentionBatchLse_dev")
@@ -953,11 +994,12 @@ class KVCache:
         n_q = q_dev.shape[1] if q_dev.dim() == 4 else 1
         old = None if old_lens is None else np.ascontiguousarray(old_lens, np.uint32)
         if (s.size != n or not (q_dev.is_contiguous() and lse_dev.is_contiguous()) or lse_dev.numel() != n * n_q * H
-                or mass_dev.shape[0] != n or not mass_dev.is_contiguous() or (old is not None and old.size != n)):
+                or mass_dev.dim() != 2 or mass_dev.shape[0] != n or not mass_dev.is_contiguous()
+                or (old is not None and old.size != n)):
             raise ValueError("attnMass_dev: contiguous q [n][n_q][H][W], lse [n][n_q][H], mass [n][positions]")
         if q_dev.shape[-1] != self.kv_rank + self.rope_dim:
             raise ValueError(f"attnMass_dev: queries of {q_dev.shape[-1]} elements")
-        _words("attnMass_dev", q_dev, lse_dev, mass_dev)
+        _reals("attnMass_dev", self.device, q_dev, lse_dev, mass_dev)
         check(lib().kvcache_attn_mass_dev(self._h, layer, n, _np_ptr(s), n_q, _dptr(q_dev), _dptr(lse_dev), H, scale,
                                           decay, None if old is None else _np_ptr(old), _dptr(mass_dev),
                                           mass_dev.shape[1], _stream(stream)), "attnMass_dev")
@@ -971,7 +1013,8 @@ class KVCache:
                 (keep_dev is not None and (keep_dev.shape != (self.n_layers, s.size, budget) or
                                            not keep_dev.is_contiguous()))):
             raise ValueError("evict_dev: contiguous mass [n_layers][n][positions], keep [n_layers][n][budget]")
-        _words("evict_dev", mass_dev, keep_dev)
+        _reals("evict_dev", self.device, mass_dev)
+        _whole("evict_dev", self.device, keep_dev)
         check(lib().kvcache_evict_dev(self._h, s.size, _np_ptr(s), budget, n_sink, n_recent, _dptr(mass_dev),
                                       mass_dev.stride(0), mass_dev.shape[2], _dptr(keep_dev), _stream(stream)),
               "evict_dev")
