@@ -1383,12 +1383,17 @@ int kvcache_attn_mass_dev(kvcache* c, uint32_t layer, uint32_t n, const uint32_t
   DevScope d(c->device);
   const cudaStream_t st = (cudaStream_t)stream;
   return guarded("kvcache_attn_mass_dev", [&]() -> int {
-    for (uint32_t b = 0; b < n; ++b)
-      if (seq_ids[b] < c->seqs.size() && c->seqs[seq_ids[b]].len > mass_stride) {
+    for (uint32_t b = 0; b < n; ++b) {
+      if (seq_ids[b] >= c->seqs.size()) {  // also one that the step's plan still lists: a load replaces them all
+        kvcu_set_error("sequence %u does not exist", seq_ids[b]);
+        return KVCU_ERR_INVALID_ARG;
+      }
+      if (c->seqs[seq_ids[b]].len > mass_stride) {
         kvcu_set_error("kvcache_attn_mass_dev: sequence %u holds %u positions, a row of sums %llu", seq_ids[b],
                        c->seqs[seq_ids[b]].len, (unsigned long long)mass_stride);
         return KVCU_ERR_INVALID_ARG;
       }
+    }
     // The plan of the step that has just appended these sequences' newest rows serves
     // as it is (its open-ended items take the row in); else that of a decode.
     const uint32_t* ids = c->d_stepu;

@@ -2,8 +2,9 @@
 import numpy as np
 import pytest
 
+from kvdata import SCALE
 from pooldata import Paged, arrays
-from test_gpu_bounded import BS, kv, make  # noqa: F401 (kv is the module's fixture)
+from test_gpu_bounded import BS, P, R, Step, kv, make  # noqa: F401 (kv is the module's fixture)
 from test_gpu_evict import want_keep
 
 pytestmark = pytest.mark.gpu
@@ -125,3 +126,22 @@ def test_a_kept_position_beyond_its_row_of_sums(kv, dims):
     want[:, :, 75:100] = 0
     cache.pool.evict_compact(0, cache.toff, cache.tables, keep, counts, mass=mass)
     assert cache.pool.status() == 0x8 and torch.equal(mass, want)
+
+
+def test_weights_of_a_sequence_that_a_load_took_away(kv, tmp_path):
+    """The step's plan still lists it; the cache has one sequence left."""
+    import torch
+
+    c = make(kv, [40, 20, 30], True, 1)
+    one = kv.KVCache.with_blocks(1, R, P, c.num_blocks, BS, quantized=True)
+    one.saveToFileV2(tmp_path / "one.ckpt")
+    st = Step(2, 6)
+    c.seq_ensure_capacity(0, 41), c.seq_ensure_capacity(2, 31)
+    st.run(c, 0, [0, 2], [40, 30], kv.Rope(P))
+    c.loadFromFileV2(tmp_path / "one.ckpt")
+    mass = torch.ones(2, 64, device="cuda")
+    with pytest.raises(kv.KVCudaError) as e:
+        c.attnMass_dev(0, [0, 2], st.q_abs, st.lse, SCALE, mass)
+    assert e.value.name == "InvalidArgument" and "sequence 2 does not exist" in str(e.value)
+    torch.cuda.synchronize()
+    assert (mass == 1).all() and c.pool().status() == 0
