@@ -613,6 +613,12 @@ int ensure_ws(kvcache* c, uint32_t n, uint32_t n_heads, uint32_t n_layers = 1) {
   return KVCU_OK;
 }
 
+// Room in d_stepu.  The kept step's plan goes by the ids in it, which do not outlive it.
+int ensure_stepu(kvcache* c, size_t n) {
+  if (c->d_stepu_cap < n) c->mla_plan_serial = ~0ull;
+  return ensure_dev(&c->d_stepu, &c->d_stepu_cap, n);
+}
+
 // The workspace, tables, lengths and plan of a batch (checked first) for layers
 // [layer, layer + n_layers); `launches` is set to those it took.
 int plan_batch(kvcache* c, uint32_t layer, uint32_t n, const uint32_t* seq_ids, uint32_t n_heads, cudaStream_t st,
@@ -713,7 +719,7 @@ int attention_batch_impl(kvcache* c, uint32_t layer, uint32_t seq, uint32_t star
   int rc = ensure_ws(c, n_pos, n_heads);
   if (!rc) rc = sync_tables(c, st);
   if (!rc) rc = sync_lens(c, st);
-  if (!rc) rc = ensure_dev(&c->d_stepu, &c->d_stepu_cap, (size_t)2 * n_pos);
+  if (!rc) rc = ensure_stepu(c, (size_t)2 * n_pos);
   if (!rc) rc = stage_acquire(c->up_rowidx, (size_t)2 * n_pos);
   if (rc) return rc;
   for (uint32_t i = 0; i < n_pos; ++i) {
@@ -760,7 +766,7 @@ int step_impl(kvcache* c, uint32_t layer, uint32_t n, const uint32_t* seq_ids, c
   // scratch: q_abs [n][H][W], rows [n][W], latent [n][H][R], lse [n][H], merge weights [n][H][3]
   const size_t q_abs_n = (size_t)n * n_heads * Wd, rows_n = (size_t)n * Wd, lat_n = (size_t)n * n_heads * R;
   rc = ensure_dev(&c->d_step, &c->d_step_cap, q_abs_n + rows_n + lat_n + (size_t)n * n_heads * 4);
-  if (!rc) rc = ensure_dev(&c->d_stepu, &c->d_stepu_cap, 3 * (size_t)n + n_seqs);
+  if (!rc) rc = ensure_stepu(c, 3 * (size_t)n + n_seqs);
   if (!rc) rc = sync_tables(c, st);
   if (!rc) rc = sync_lens(c, st);
   if (!rc) rc = ensure_ws(c, n, n_heads);

@@ -4,8 +4,9 @@ import pytest
 
 from kvdata import SCALE
 from pooldata import Paged, arrays
-from test_gpu_bounded import BS, P, R, Step, kv, make  # noqa: F401 (kv is the module's fixture)
+from test_gpu_bounded import BS, Cached, P, R, Step, kv, make  # noqa: F401 (kv is the module's fixture)
 from test_gpu_evict import want_keep
+from test_gpu_mass import check, want_mass
 
 pytestmark = pytest.mark.gpu
 
@@ -145,3 +146,26 @@ def test_weights_of_a_sequence_that_a_load_took_away(kv, tmp_path):
     assert e.value.name == "InvalidArgument" and "sequence 2 does not exist" in str(e.value)
     torch.cuda.synchronize()
     assert (mass == 1).all() and c.pool().status() == 0
+
+
+def test_weights_after_a_refused_step_of_a_larger_cache(kv):
+    """The refused step needed more room for its ids; the plan of the step before goes by its own."""
+    import torch
+
+    lens = [40, 20]
+    c = make(kv, lens, True, 1)
+    st = Step(2, 6)
+    for s in range(2):
+        c.seq_ensure_capacity(s, lens[s] + 1)
+    st.run(c, 0, [0, 1], lens, kv.Rope(P))
+    for _ in range(5000):
+        c.seq_create()
+    with pytest.raises(kv.KVCudaError):
+        Step(2, 7).run(c, 0, [0, 0], [41, 41], kv.Rope(P))
+    lens = [41, 21]
+    before = torch.ones(2, 64, device="cuda")
+    mass = before.clone()
+    c.attnMass_dev(0, [0, 1], st.q_abs, st.lse, SCALE, mass)
+    assert c.pool().status() == 0
+    want, tol = want_mass(Cached(c, lens), [0, 1], st.q_abs[:, None], st.lse[:, None], before, 1.0, lens)
+    check(mass, want, tol)
