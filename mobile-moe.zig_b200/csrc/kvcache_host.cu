@@ -1406,7 +1406,15 @@ int kvcache_attn_mass_dev(kvcache* c, uint32_t layer, uint32_t n, const uint32_t
     uint32_t launches = 0;
     bool step_plan = c->ws && c->mla_plan_serial == c->plan_serial && c->mla_plan_ids.size() == n &&
                      std::equal(c->mla_plan_ids.begin(), c->mla_plan_ids.end(), seq_ids);
-    for (uint32_t b = 0; step_plan && b < n; ++b) step_plan = c->seqs[seq_ids[b]].len >= c->mla_plan_hist[b];
+    // Grown much beyond the step's own rows, the plan's last items would hold the growth alone
+    // (plan_batch's rule).
+    uint64_t planned = 0, held = 0;
+    for (uint32_t b = 0; step_plan && b < n; ++b) {
+      planned += c->mla_plan_hist[b];
+      held += c->seqs[seq_ids[b]].len;
+      step_plan = c->seqs[seq_ids[b]].len >= c->mla_plan_hist[b];
+    }
+    step_plan = step_plan && held <= planned + n + planned / 8;
     int rc = KVCU_OK;
     if (step_plan) {
       rc = sync_tables(c, st);
