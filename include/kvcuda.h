@@ -302,9 +302,9 @@ int kvcu_decode_ws_set_impl(kvcu_decode_ws* ws, int impl);
 /* Every wait of the tensor-core decode and attention-mass kernels is bounded: after `cycles` SM
  * clocks (0 = the default, 2^31, about a second at 1.9 GHz) the CTA records
  * KVCU_STATUS_TIMEOUT in the pool's status word, all its roles unwind, its
- * in-flight copies and MMAs are waited for (with the same bound) and its TMEM
- * is released, so the context stays usable and the host reads the error.  At
- * most 2^40. */
+ * in-flight copies and MMAs are waited for (with the same bound; the
+ * attention-mass kernels with the default one) and its TMEM is released, so the
+ * context stays usable and the host reads the error.  At most 2^40. */
 int kvcu_decode_ws_set_wait_limit(kvcu_decode_ws* ws, uint64_t cycles);
 /* Test hook for that unwind, needing no GPU fault: in the tensor-core kernel,
  * every CTA's producer skips the copy and the arrival of the first slice of

@@ -282,14 +282,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         tile->flags = 0;
         kvtc::mbar_arrive(bar(M::B_TF));
       }
-      if (!ok) {
-        // the copies in flight must land before the CTA leaves: the last of each slot, and the last scales
-        const long long t0 = clock64();
-        while (sent && !kvtc::mbar_try(bar(M::B_UF + (int)lane), (sent - 1) & 1u) && clock64() - t0 <= DRAIN_LIMIT) {
-        }
-        __syncwarp();
-        while (ti && !kvtc::mbar_try(bar(M::B_TF), (ti - 1) & 1u) && clock64() - t0 <= DRAIN_LIMIT) {
-        }
+      // The copies in flight must land before the CTA leaves, also where only their readers have given up: the
+      // last of each slot, and the last scales (which a tile that was handed back has had).
+      const long long t0 = clock64();
+      while (sent && !kvtc::mbar_try(bar(M::B_UF + (int)lane), (sent - 1) & 1u) && clock64() - t0 <= DRAIN_LIMIT) {
+      }
+      __syncwarp();
+      while (!ok && ti && !kvtc::mbar_try(bar(M::B_TF), (ti - 1) & 1u) && clock64() - t0 <= DRAIN_LIMIT) {
       }
     } else if (warp < ISSUER + 2) {
       // -------------------------------------------------------------- MMA issuers, one per pair

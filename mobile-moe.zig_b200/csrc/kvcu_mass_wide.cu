@@ -236,16 +236,15 @@ __global__ void __launch_bounds__(THREADS, 1) k_mass_wide(const Wide t) {
         }
       }
     }
-    if (!ok) {  // the copies in flight must land before the CTA leaves
-      const long long t0 = clock64();
-      while (sent && !kvtc::mbar_try(bar(B_BF + lane), (sent - 1) & 1u) && clock64() - t0 <= DRAIN_LIMIT) {
-      }
-      __syncwarp();
-      while (unit && !kvtc::mbar_try(bar(B_CF + ((unit - 1) & 1u)), ((unit - 1) >> 1) & 1u) &&
-             clock64() - t0 <= DRAIN_LIMIT) {
-      }
-      __syncwarp();
+    // the copies in flight must land before the CTA leaves, also where only their readers have given up
+    const long long t0 = clock64();
+    while (sent && !kvtc::mbar_try(bar(B_BF + lane), (sent - 1) & 1u) && clock64() - t0 <= DRAIN_LIMIT) {
     }
+    __syncwarp();
+    while (unit && !kvtc::mbar_try(bar(B_CF + ((unit - 1) & 1u)), ((unit - 1) >> 1) & 1u) &&
+           clock64() - t0 <= DRAIN_LIMIT) {
+    }
+    __syncwarp();
   } else if (warp == ISSUER || warp == ISSUER + 1) {
     // ---------------------------------------------------------------- MMA issuers
     // Few MMAs queue up behind the running one, not enough for the time that a warp's waits take: two
