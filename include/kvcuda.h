@@ -628,6 +628,9 @@ int kvcache_mla_step_dev(kvcache* c, uint32_t layer, uint32_t n, const uint32_t*
                          const float* v_b_dev, uint32_t n_heads, uint32_t qk_nope, uint32_t v_dim,
                          float scale, float* attn_dev, void* stream);
 /* ---- a bounded cache (no counterpart in the reference) ----
+ * The step, the weights and the eviction keep lengths, tables and blocks on the
+ * host: on a stream that is being captured they return KVCU_ERR_UNSUPPORTED
+ * (kvcu_attn_mass, kvcu_evict_* and kvcu_rope_apply can be captured).
  * The step above with the rotary frequencies of `rope` at rope_positions[b] (host;
  * NULL: the cache positions): in a cache that evicts, a token's position runs on
  * while its row goes to the next free place.  q_abs_dev [n][H][R+P] and lse_dev

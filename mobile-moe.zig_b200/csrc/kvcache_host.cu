@@ -849,6 +849,16 @@ int guarded(const char* what, F f) {
   }
 }
 
+// The bounded cache's calls change lengths, tables and blocks on the host, and their uploads
+// read what the host writes later: a graph could not repeat them.
+int refuse_capture(const char* what, cudaStream_t st) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  KVCU_CUDA(cudaStreamIsCapturing(st, &status));
+  if (status == cudaStreamCaptureStatusNone) return KVCU_OK;
+  kvcu_set_error("%s: the stream is being captured into a graph (capture the kvcu_* calls instead)", what);
+  return KVCU_ERR_UNSUPPORTED;
+}
+
 // The bounded cache's device scratch: `words` of it for a call on `st`, after the
 // call before (on whichever stream) is through with it.
 int bound_acquire(kvcache* c, size_t words, size_t staged, cudaStream_t st) {
@@ -1365,7 +1375,10 @@ int kvcache_mla_step_rope_dev(kvcache* c, uint32_t layer, uint32_t n, const uint
     kvcu_set_error("kvcache_mla_step_rope_dev: the absorbed queries are not 16-byte aligned");
     return KVCU_ERR_INVALID_ARG;
   }
-  return guarded("kvcache_mla_step_rope_dev", [&] {
+  return guarded("kvcache_mla_step_rope_dev", [&]() -> int {
+    DevScope d(c->device);
+    const int rc = refuse_capture("kvcache_mla_step_rope_dev", (cudaStream_t)stream);
+    if (rc) return rc;
     return step_impl(c, layer, n, seq_ids, positions, rope, rope_positions, q_dev, kv_a_dev, norm_w_dev, eps, 0.0f,
                      k_b_dev, v_b_dev, n_heads, qk_nope, v_dim, scale, attn_dev, q_abs_dev, lse_dev, stream);
   });
@@ -1389,6 +1402,8 @@ int kvcache_attn_mass_dev(kvcache* c, uint32_t layer, uint32_t n, const uint32_t
   DevScope d(c->device);
   const cudaStream_t st = (cudaStream_t)stream;
   return guarded("kvcache_attn_mass_dev", [&]() -> int {
+    int rc = refuse_capture("kvcache_attn_mass_dev", st);
+    if (rc) return rc;
     for (uint32_t b = 0; b < n; ++b) {
       if (seq_ids[b] >= c->seqs.size()) {  // also one that the step's plan still lists: a load replaces them all
         kvcu_set_error("sequence %u does not exist", seq_ids[b]);
@@ -1415,7 +1430,6 @@ int kvcache_attn_mass_dev(kvcache* c, uint32_t layer, uint32_t n, const uint32_t
       step_plan = c->seqs[seq_ids[b]].len >= c->mla_plan_hist[b];
     }
     step_plan = step_plan && held <= planned + n + planned / 8;
-    int rc = KVCU_OK;
     if (step_plan) {
       rc = sync_tables(c, st);
       if (!rc) rc = sync_lens(c, st);
@@ -1453,6 +1467,8 @@ int kvcache_evict_dev(kvcache* c, uint32_t n, const uint32_t* seq_ids, uint32_t 
   DevScope d(c->device);
   const cudaStream_t st = (cudaStream_t)stream;
   return guarded("kvcache_evict_dev", [&]() -> int {
+    int rc = refuse_capture("kvcache_evict_dev", st);
+    if (rc) return rc;
     const uint64_t mass_row = kvcu_mass_row(c->n_layers, n, mass_layer_stride, mass_stride);
     if (!mass_row) {
       kvcu_set_error("kvcache_evict_dev: rows of sums overlap at strides %llu (layers) and %llu (sequences)",
@@ -1503,7 +1519,7 @@ int kvcache_evict_dev(kvcache* c, uint32_t n, const uint32_t* seq_ids, uint32_t 
       return KVCU_ERR_OUT_OF_BLOCKS;
     }
     const size_t list = keep_dev ? 0 : (size_t)c->n_layers * n * budget;
-    int rc = bound_acquire(c, 2 * (size_t)n + list, n, st);
+    rc = bound_acquire(c, 2 * (size_t)n + list, n, st);
     if (!rc)
       rc = rewritten([&](uint32_t s, uint32_t bi) -> int {
         const uint32_t pos = bi * c->block_size;

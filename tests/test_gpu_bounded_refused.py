@@ -169,3 +169,31 @@ def test_weights_after_a_refused_step_of_a_larger_cache(kv):
     assert c.pool().status() == 0
     want, tol = want_mass(Cached(c, lens), [0, 1], st.q_abs[:, None], st.lse[:, None], before, 1.0, lens)
     check(mass, want, tol)
+
+
+def test_on_a_stream_that_is_being_captured(kv):
+    """The cache's calls keep state on the host, which a graph would not repeat."""
+    import torch
+
+    c, t = shared(kv, 8)
+    st, rope = Step(1, 6), kv.Rope(P)
+    mass, keep = torch.rand(2, 1, 96, device="cuda"), torch.empty(2, 1, 96, dtype=torch.int32, device="cuda")
+    c.evict_dev([1], 96, mass, keep_dev=keep)  # within the budget: kernels loaded, scratch there
+    before, kept = state(c, t), mass.clone()
+    c.seq_truncate(1, 95)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        s = torch.cuda.current_stream()
+        for f in (lambda: c.evict_dev([1], 64, mass, stream=s), lambda: c.evict_dev([0], 64, mass, keep_dev=keep[:, :, :64].contiguous(), stream=s),
+                  lambda: c.attnMass_dev(0, [1], st.q_abs, st.lse, SCALE, mass[0], old_lens=[95], stream=s),
+                  lambda: st.run(c, 0, [1], [95], rope, stream=s)):
+            with pytest.raises(kv.KVCudaError) as e:
+                f()
+            assert e.value.name == "Unsupported", e.value
+    del graph
+    st.run(c, 0, [0], [95], rope)
+    assert c.seq_len(0) == 96 and c.seq_len(1) == 95
+    assert [c.seq_block_table(s) for s in range(2)] != before[0]  # the step copied the block it wrote into
+    assert torch.equal(mass, kept)
+    c.evict_dev([1], 64, mass)
+    assert c.seq_len(1) == 64 and c.pool().status() == 0
