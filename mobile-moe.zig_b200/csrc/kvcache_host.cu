@@ -1449,7 +1449,7 @@ int kvcache_attn_mass_dev(kvcache* c, uint32_t layer, uint32_t n, const uint32_t
                         mass_dev, mass_stride, st);
     if (old_lens) KVCU_CUDA(cudaEventRecord(c->bound_done, st));
     if (rc) return rc;
-    c->last_launches = launches + 1;
+    c->last_launches = launches + c->ws->mass_launches;
     return KVCU_OK;
   });
 }

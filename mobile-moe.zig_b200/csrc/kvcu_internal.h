@@ -54,6 +54,7 @@ struct kvcu_decode_ws {
   uint64_t wait_limit;         // clocks a bounded device wait may take (0: the default, ~2^31)
   uint32_t withhold_plus1;     // test hook: 0, or 1 + the tile whose first slice the producer withholds
   uint32_t last_launches;
+  uint32_t mass_launches;      // of the last kvcu_attn_mass
   int num_sms;
   int decode_ctas;           // resident decode CTAs (grid of the persistent kernel)
   int impl;                  // KVCU_DECODE_AUTO / _CUDA_CORE / _TENSOR_CORE

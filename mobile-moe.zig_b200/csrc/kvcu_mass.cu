@@ -728,6 +728,7 @@ extern "C" int kvcu_attn_mass(kvcu_decode_ws* ws, kvcu_pool* pool, uint32_t laye
     kvcu_set_error("kvcu_attn_mass: %llu rows, TMA coordinates reach 2^31 - 1", (unsigned long long)pool->rows());
     return KVCU_ERR_UNSUPPORTED;
   }
+  ws->mass_launches = 1;
   if (!pool->quantized) return launch_chunks<false>(pool, a, ws, st);
   // Many columns: the wide kernel, in as few passes over the queries as the workspace's
   // decode partials (idle outside a decode) hold their parts for.
@@ -735,7 +736,9 @@ extern "C" int kvcu_attn_mass(kvcu_decode_ws* ws, kvcu_pool* pool, uint32_t laye
   uint32_t passes = 1, count = n_q;
   while (count * n_heads >= WIDE_MIN_COLS && wide_scratch(n, count * n_heads) > room) count = (n_q + passes) / (passes + 1), ++passes;
   if (count * n_heads < WIDE_MIN_COLS) return launch_chunks<true>(pool, a, ws, st);
+  ws->mass_launches = 0;
   for (uint32_t q0 = 0; q0 < n_q; q0 += count) {
+    ws->mass_launches += 2;  // the columns' parts, and the sums
     const int rc = launch_wide(pool, a, q0, n_q - q0 < count ? n_q - q0 : count, ws->part_o, ws, st);
     if (rc) return rc;
   }

@@ -1,4 +1,4 @@
-"""The weights of sequences that grew between a step and the call."""
+"""The launches of the weights: sequences that grew between a step and the call, windows of queries."""
 import numpy as np
 import pytest
 
@@ -32,3 +32,16 @@ def test_the_steps_plan_serves_while_the_batch_grew_little(kv, grown, launches):
     assert c.last_launches == launches
     assert c.pool().status() == 0
     check(mass, want, tol)
+
+
+@pytest.mark.parametrize("quant,n_q,launches", [(True, 1, 1), (True, 2, 1), (True, 3, 2), (True, 40, 2), (False, 40, 1)])
+def test_launches_of_a_window(kv, quant, n_q, launches):
+    """Many columns of Q8_0 rows are laid out first; a plan, where the batch is another one, comes on top."""
+    import torch
+
+    c = make(kv, [300], quant, 1)
+    q = torch.randn(1, n_q, 20, W, device="cuda") * 0.05
+    mass, lse = torch.zeros(1, 300, device="cuda"), torch.zeros(1, n_q, 20, device="cuda")
+    for plan in (1, 0):
+        c.attnMass_dev(0, [0], q, lse, SCALE, mass)
+        assert c.last_launches == launches + plan
