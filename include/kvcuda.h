@@ -367,7 +367,8 @@ int kvcu_mla_decode_noalloc(kvcu_pool* pool, uint32_t layer, uint32_t n, const u
  * rows appended since the last call need no zeroing.  Positions >= len are left
  * as they were; a length beyond the table or mass_stride sets
  * KVCU_STATUS_BAD_LEN and is cut, a bad block sets KVCU_STATUS_BAD_BLOCK and its
- * positions are left.  Entries may share a sequence (each has its own sums).
+ * positions are left.  Entries may share a sequence (each has its own sums).  An
+ * infinity or NaN in a row makes that row's sum infinite or NaN, and no other's.
  * Runs on the last one-layer plan of `ws` (kvcu_decode_plan or _causal; the
  * batch must be the one planned), so a step's decode and its mass share it; for
  * many columns (n_q * n_heads) of Q8_0 rows it also uses the workspace's decode
@@ -422,8 +423,9 @@ int kvcu_evict_compact(kvcu_pool* pool, uint32_t layer, uint32_t n_layers, uint3
  *             KVCU_ROPE_NTK     base * factor^(rot_dim/(rot_dim-2)) in place of base
  *             KVCU_ROPE_YARN    f_i / factor for pairs that turn less than beta_slow
  *                               times over orig_ctx positions, f_i for those that turn
- *                               more than beta_fast times, a linear ramp over the pairs
- *                               between (YaRN, Peng et al. 2023)
+ *                               more than beta_fast times, between them a ramp linear in
+ *                               the pair's index (YaRN, Peng et al. 2023, with the ramp of
+ *                               the authors' code; the paper's is over the turns)
  *   base > 1, factor >= 1; beta_fast / beta_slow: 0 = 32 / 1
  *   mscale    magnitude m; 0 = 0.1 ln(factor) + 1 with YARN, else 1
  * kvcu_rope_create returns NULL (and sets the last error) on anything else. */

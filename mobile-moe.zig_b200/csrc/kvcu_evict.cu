@@ -6,10 +6,15 @@
 //   masses' 32-bit order (11 + 11 + 10 bits): the row is read once into shared
 //   memory while the first histogram is formed, the other passes run there.
 //   Floor: one read of the masses (4 B per position); bound: the instructions of three
-//   passes.  512 rows of 1.5k to 65k positions, 2,048 kept: 57 us (35.9 MB read once).
+//   passes, and the longest row, which one CTA has alone where there are more rows than
+//   SMs (64,784 positions, as many as an SM's whole share).  512 rows of 1.5k to 65k
+//   positions, 2,048 kept: 57 us (35.9 MB read once).  The first pass has four bins to an
+//   octave: masses that all lie within one or two octaves share a few bins, whose atomics
+//   collide and whose keys overflow the list, 101 us for the same rows.
 // k_evict_compact: row j of a sequence := its row keep[j], in place through the
 //   block table, in every layer, and the masses with it.  Bound: one read and
-//   one write of the kept rows.  512 pairs of 2,048 rows of 612 B: 252 us, 4.3 TB/s.
+//   one write of the kept rows.  512 pairs of 2,048 rows of 612 B: 252 us, 4.3 TB/s; of
+//   2,304 B (f32): 128 pairs 372 us, 256 pairs 725 us, 3.3 TB/s.
 #include <cuda_runtime.h>
 
 #include "kvcu_internal.h"

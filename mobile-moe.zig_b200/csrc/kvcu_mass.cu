@@ -46,10 +46,15 @@ namespace {
 //                through rings, and each tile's description and scales
 //   warps 17-18  issue the MMAs, one for each pair
 // More columns (queries x heads) than an instance has go in chunks: the item's rows
-// are streamed again, from L2, for each (Q8_0 rows only below 48 columns: kvcu_mass_wide.cu).
-// Bound: instructions.  Of 46 clocks a Q8_0 row and SM the loads alone take 28 (6.2 TB/s),
-// unpacking and the finish most of the rest.  Measured with 20 heads: 64 sequences to 32k
-// rows 68 us (3.0 TB/s), 192 to 65k 379 us (3.5 TB/s), one of 640 rows 10.8 us; f32, 16
+// are streamed again for each, from L2 where all items' rows fit there, else from memory
+// (Q8_0 rows only below 48 columns: kvcu_mass_wide.cu).  192 sequences of 2.0M rows in all:
+// 336 us with 20 heads, 608 us with 32 (two chunks); f32, 16 sequences of 8,000 rows: 77 us
+// for one query of 20 heads, 389 us for eight (seven chunks).
+// Bound: waits.  A Q8_0 row takes an SM 46 clocks, where the loads alone take 28 (6.2 TB/s)
+// and issuing its 98 warp instructions 24.5: no pipe is saturated (issue 48%, memory 35%,
+// tensor 18%), and each of a warpgroup's nine steps waits for its TMEM stores, for the MMAs
+// of the step before and for their sums.  Measured with 20 heads: 64 sequences to 32k rows
+// 68-69 us (3.0 TB/s), 192 to 65k 392 us (3.4 TB/s), one of 777 rows 10.8 us; f32, 16
 // sequences to 8k 43 us, 64 of 8,192 rows 6.0-6.2 TB/s.
 constexpr int COMPUTE = 16, PRODUCER = 16, ISSUER = 17;  // warps; two issuers
 constexpr int TC_THREADS = (COMPUTE + 4) * 32;

@@ -19,8 +19,10 @@
 // Bound: memory.  Each CTA forms the sines of its tokens once in shared memory
 // (a few 64-bit operations per token and pair, shared by all heads), then every
 // thread turns V pairs with two 16-byte loads and two 16-byte stores.
-// Measured: 4,096 tokens' gradient in f32 (40 heads of 128) 33 us, 5.1 TB/s; a bf16 prompt
-// 14 us; one token is the launch.
+// Measured: 4,096 tokens' gradient in f32 (40 heads of 128) 33 us, 5.1 TB/s; one token is
+// the launch.  A bf16 prompt of 8,191 tokens takes 14 us, 3.1 TB/s, by latency (issue 39%,
+// memory 19%): no row is being loaded until a CTA's sines are there, and after that each
+// thread has two loads in flight.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -217,7 +219,9 @@ extern "C" kvcu_rope* kvcu_rope_create(const kvcu_rope_desc* d) {
   if (d->scaling == KVCU_ROPE_NTK) base *= pow(d->factor, dim / (dim - 2.0));
   double low = 0.0, high = 0.0;
   if (d->scaling == KVCU_ROPE_YARN) {
-    // the pair that makes `turns` full turns over the trained context
+    // the pair that makes `turns` full turns over the trained context; the ramp between the two is linear in
+    // the pair's index, as the method's authors' code and the models trained with it have it (their paper
+    // describes one over the number of turns)
     auto pair_of = [&](double turns) { return dim * log(d->orig_ctx / (turns * 2.0 * pi)) / (2.0 * log(base)); };
     low = fmax(floor(pair_of(fast)), 0.0);
     high = fmin(ceil(pair_of(slow)), dim - 1.0);
