@@ -1469,12 +1469,7 @@ int kvcache_evict_dev(kvcache* c, uint32_t n, const uint32_t* seq_ids, uint32_t 
   return guarded("kvcache_evict_dev", [&]() -> int {
     int rc = refuse_capture("kvcache_evict_dev", st);
     if (rc) return rc;
-    const uint64_t mass_row = kvcu_mass_row(c->n_layers, n, mass_layer_stride, mass_stride);
-    if (!mass_row) {
-      kvcu_set_error("kvcache_evict_dev: rows of sums overlap at strides %llu (layers) and %llu (sequences)",
-                     (unsigned long long)mass_layer_stride, (unsigned long long)mass_stride);
-      return KVCU_ERR_INVALID_ARG;
-    }
+    const uint64_t mass_row = kvcu_mass_row(c->n_layers, n, mass_layer_stride, mass_stride);  // 0: they overlap
     std::vector<char> seen(c->seqs.size(), 0);
     bool any = false;
     for (uint32_t b = 0; b < n; ++b) {
@@ -1485,8 +1480,9 @@ int kvcache_evict_dev(kvcache* c, uint32_t n, const uint32_t* seq_ids, uint32_t 
       }
       seen[s] = 1;
       if (c->seqs[s].len > mass_row) {
-        kvcu_set_error("kvcache_evict_dev: sequence %u holds %u positions, a row of sums %llu", s, c->seqs[s].len,
-                       (unsigned long long)mass_row);
+        kvcu_set_error("kvcache_evict_dev: sequence %u holds %u positions, a row of sums %llu at strides %llu (layers) "
+                       "and %llu (sequences)", s, c->seqs[s].len, (unsigned long long)mass_row,
+                       (unsigned long long)mass_layer_stride, (unsigned long long)mass_stride);
         return KVCU_ERR_INVALID_ARG;
       }
       any = any || c->seqs[s].len > budget;

@@ -99,6 +99,15 @@ def test_rows_of_sums_that_overlap(kv):
     assert torch.equal(mass, kept) and all(torch.equal(a, b) for a, b in zip(arrays(cache.pool), before))
 
 
+def test_sums_of_empty_sequences_may_have_no_room(kv):
+    import torch
+
+    c = make(kv, [0, 0], True, 2)
+    ids, some = np.array([0, 1], np.uint32), torch.zeros(1, device="cuda")
+    assert kv.lib().kvcache_evict_dev(c._h, 2, ids.ctypes.data, 8, 0, 0, some.data_ptr(), 0, 0, None, None) == 0
+    assert c.last_launches == 0 and c.seq_len(0) == 0
+
+
 def test_sums_with_the_layers_inside_the_entries(kv):
     """[entry][layer][position] is a layout of its own, and one entry's rows may be any distance apart."""
     import torch
